@@ -132,6 +132,63 @@ int mv_op_gemm(void* stream, int32_t M, int32_t N, int32_t K, const void* a, con
 int mv_op_attention_rows(void* stream, int32_t batch, int32_t T, int32_t n_head, int32_t head_dim, int32_t causal, const void* qkv,
                          void* out);
 
+/* ---- microscaled 4-bit floating point (MXFP4) on caller-owned DEVICE buffers.  No reference equivalent: the 4-bit format that the MI355X
+ * matrix cores multiply directly, beside the reference's int4 weights.  The three entries below enqueue work on `stream` and return: no
+ * allocation, no scratch memory, no synchronisation (they may be captured into a graph).
+ * Format: a row of K values in nb = ceil(K / 32) blocks of 32 columns; a block is 32 codes of 4 bits (sign, 2 exponent bits, 1 mantissa bit:
+ * 0 0.5 1 1.5 2 3 4 6) times 2^(s - 127), s its scale byte; s = 255: NaN.
+ *   codes  [rows][16 nb] bytes (column 2j low, 2j + 1 high nibble of byte j; zero past K), 16-byte aligned;   scales [rows][nb] bytes
+ * A call with no row or no column (M, N or rows 0) does nothing.  Sizes and strides count elements; strides need no alignment, but 16-byte
+ * aligned rows are read fastest.
+ *
+ * mv_op_quantize_mxfp4: w [N][ldw], dtype MV_BF16 or MV_F32 -> codes, scales and, when not NULL, the values they stand for as bf16 [N][K]
+ * (`dequantised` may be w itself when w is bf16 and ldw = K).  Block exponent floor(log2 max|w|) - 2, at least -127; codes rounded to nearest,
+ * ties to even, beyond 6 to 6; a block with an infinity or a NaN is NaN. */
+int mv_op_quantize_mxfp4(void* stream, int32_t N, int32_t K, int32_t dtype, const void* w, int64_t ldw, void* codes, void* scales,
+                         void* dequantised);
+/* out[M][N] = x . W^T + bias, with codes2 / scales2 the gated pair silu(x . W^T + bias) * (x . W2^T + bias2); then + residual.  x bf16 [M][ldx];
+ * W, W2 MXFP4 [N][K]; bias, bias2 bf16 [N] or NULL; residual [M][N] of the output's type or NULL (may be `out` itself); out_dtype MV_BF16 or
+ * MV_F32.  The weights enter the matrix cores as bf16 (exact), sums are fp32, the result is rounded once. */
+int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x, int64_t ldx, const void* codes, const void* scales,
+                       const void* codes2, const void* scales2, const void* bias, const void* bias2, const void* residual, int32_t out_dtype,
+                       void* out);
+/* The same with x in MXFP4 too (codes [M][16 nb], scales [M][nb]): scaled matrix instructions on the codes themselves. */
+int mv_op_gemm_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x_codes, const void* x_scales, const void* codes,
+                     const void* scales, const void* codes2, const void* scales2, const void* bias, const void* bias2, const void* residual,
+                     int32_t out_dtype, void* out);
+
+/* Controls on next-token logits before the sampler (no reference equivalent).  The struct lies on the host, its pointers are DEVICE buffers;
+ * NULL switches a control off. */
+typedef struct mv_logit_controls {
+    const float* guidance;       /* [rows] g, needed when `uncond` is given                                             */
+    const float* repetition;     /* [rows] tokens of the history: x > 0 ? x / repetition : x * repetition                */
+    const float* presence;       /* [rows] subtracted once from tokens that occur behind the prompt                      */
+    const float* frequency;      /* [rows] subtracted once per occurrence behind the prompt                              */
+    const int32_t* history;      /* [rows][ld_history] token ids, prompt first; ids outside the vocabulary are ignored   */
+    const int32_t* history_len;  /* [rows] ids in use, clamped to 0 .. history_cap; NULL: history_cap                    */
+    const int32_t* prompt_len;   /* [rows] how many of them are the prompt; NULL: 0                                      */
+    int64_t ld_history;
+    int32_t history_cap;
+    int32_t n_bias;              /* entries per row                                                                     */
+    const int32_t* bias_ids;     /* [rows][ld_bias] token ids; ids outside the vocabulary (-1) are no entries, of an id given twice
+                                    the later entry holds                                                               */
+    const float* bias;           /* [rows][ld_bias] added                                                               */
+    int64_t ld_bias;             /* 0: one list for all rows                                                            */
+    const uint32_t* masks;       /* [n_masks][ld_mask] words, token v = bit v % 32 of word v / 32: 0 forbids it           */
+    const int32_t* mask_index;   /* [rows] the row's mask, outside 0 .. n_masks - 1: none; NULL: mask r for row r         */
+    int64_t ld_mask;
+    int32_t n_masks;
+    int32_t pad0;
+} mv_logit_controls;
+/* logits (and uncond) [rows][ld], dtype MV_BF16 or MV_F32 -> out [rows][ld_out] of out_dtype; per token, in fp32, rounded once:
+ *   with uncond: x = g x + (1 - g) u (an x of -inf stays);  repetition, then - (n frequency + presence);  + bias;  mask bit 0: -inf, NaN or not.
+ * An engine's [2u] conditioned, [2u + 1] unconditioned rows are logits, uncond = logits + vocab, ld = 2 vocab.  `out` may be `logits` (same dtype
+ * and stride).  allowed (optional) [rows]: tokens the mask leaves, 0 when a grammar has run into a dead end (the row is -inf throughout).
+ * Enqueued on `stream`: no allocation, no scratch memory, no synchronisation.  out feeds mv_op_sample with a row of zeros as the unconditioned
+ * logits, guidance_scale 1, one_minus_guidance 0. */
+int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, int32_t dtype, const void* logits, const void* uncond, int64_t ld,
+                         const mv_logit_controls* controls, int32_t out_dtype, void* out, int64_t ld_out, int32_t* allowed);
+
 /* Roofline probe: launches one kernel kind of the decode step `iters` times back to back on the engine stream, cycling
  * through the layers' weights (so the stream is HBM-cold: 24 x 46 MB >> the 256 MB Infinity Cache), bracketed by HIP
  * events on that stream.  Returns the average launch duration and the ALGORITHMIC bytes one launch must move

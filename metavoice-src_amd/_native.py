@@ -66,6 +66,15 @@ class mv_sampling(C.Structure):
     ]
 
 
+class mv_logit_controls(C.Structure):
+    _fields_ = [
+        ("guidance", C.c_void_p), ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p), ("history", C.c_void_p),
+        ("history_len", C.c_void_p), ("prompt_len", C.c_void_p), ("ld_history", C.c_int64), ("history_cap", C.c_int32), ("n_bias", C.c_int32),
+        ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("ld_bias", C.c_int64), ("masks", C.c_void_p), ("mask_index", C.c_void_p),
+        ("ld_mask", C.c_int64), ("n_masks", C.c_int32), ("pad0", C.c_int32),
+    ]
+
+
 # every symbol include/metavoice_hip.h declares: (name, restype, argtypes)
 _P = C.c_void_p
 SYMBOLS = [
@@ -91,6 +100,10 @@ SYMBOLS = [
     ("mv_op_gemv_int4", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, C.c_float, _P, _P]),
     ("mv_op_gemm", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, C.c_int32, _P]),
     ("mv_op_attention_rows", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P]),
+    ("mv_op_quantize_mxfp4", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P]),
+    ("mv_op_linear_mxfp4", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P, _P, _P, _P, _P, C.c_int32, _P]),
+    ("mv_op_gemm_mxfp4", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int32, _P]),
+    ("mv_op_logit_controls", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int64, C.POINTER(mv_logit_controls), C.c_int32, _P, C.c_int64, _P]),
     ("mv_stage2_create", C.c_int, [C.POINTER(mv_stage2_config), C.POINTER(_P)]),
     ("mv_stage2_destroy", C.c_int, [_P]),
     ("mv_stage2_load_weight", C.c_int, [_P, C.c_char_p, _P, C.c_int32, C.c_int64, C.c_int64]),

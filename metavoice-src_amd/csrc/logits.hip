@@ -1,0 +1,222 @@
+// Controls on next-token logits, before the sampler: guidance mix, penalties for repeated tokens, biases, grammar masks.
+//
+// For token v of a row, in fp32, rounded once at the end:
+//   x = logits[v]                                     with `uncond`: -inf stays, else g * logits[v] + (1 - g) * uncond[v]
+//   v occurs in the history:                          x = x > 0 ? x / repetition : x * repetition
+//   v occurs n > 0 times behind the prompt:           x = x - (n * frequency + presence)
+//   v is in the bias list (its last entry holds):     x = x + bias
+//   the row's mask has bit v clear:                   x = -inf, whatever stood there (NaN and infinities too)
+//
+// Split: one workgroup takes LC_CHUNK consecutive tokens of one row and keeps two words per token in LDS, the count from the history and the number of
+// the bias entry that holds.  It scans the whole history and bias list of its row and keeps what falls into its chunk: a history is short beside the
+// row (and comes from the L2 for all chunks but the first), so this replaces a count array in memory, a launch that clears it and one that fills it.
+// Integer adds, ors and maxima in LDS give the same words in any order: results do not depend on timing.  Bound by memory when rows x vocab is large,
+// by the latency of one launch with two dependent loads (length, then history) when it is not.
+#include "common.h"
+#include "op_common.h"
+
+#define LC_THREADS 512
+#define LC_GROUPS 2                                // groups of 4 consecutive tokens per thread
+#define LC_CHUNK (LC_THREADS * LC_GROUPS * 4)      // 4096 tokens: two words each are 32 KB of LDS
+
+#define LC_TRY(expr)                                                                                                               \
+    do {                                                                                                                           \
+        hipError_t _e = (expr);                                                                                                    \
+        if (_e != hipSuccess) return mv_fail(MV_ERR_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(_e), __FILE__, __LINE__); \
+    } while (0)
+
+namespace {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef f32x4_t f32x4_any __attribute__((aligned(4)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+
+struct ControlArgs {
+    mv_logit_controls c;
+    const void* logits;
+    const void* uncond;
+    void* out;
+    int32_t* allowed;
+    int64_t ld, ld_out;
+    int32_t vocab;
+    uint32_t chunks;  // per row
+};
+
+// 4 consecutive logits of a row from token v on, zero past the vocabulary
+template <bool F32>
+__device__ __forceinline__ f32x4_t lc_load(const void* base, int64_t at, int left) {
+    f32x4_t r = {0, 0, 0, 0};
+    if (F32) {
+        const float* p = (const float*)base + at;
+        if (left >= 4) return *(const f32x4_any*)p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) r[i] = p[i];
+    } else {
+        const bf16_t* p = (const bf16_t*)base + at;
+        if (left >= 4) {
+            const u32x2 q = *(const u32x2_any*)p;
+            return f32x4_t{bf_lo(q[0]), bf_hi(q[0]), bf_lo(q[1]), bf_hi(q[1])};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) r[i] = bf2f(p[i]);
+    }
+    return r;
+}
+
+template <bool IN32, bool OUT32>
+__global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const ControlArgs a) {
+    __shared__ __attribute__((aligned(16))) uint32_t count[LC_CHUNK];  // bit 31: in the prompt; below: occurrences behind it
+    __shared__ __attribute__((aligned(16))) uint32_t entry[LC_CHUNK];  // 1 + the bias entry that holds, 0: none
+    __shared__ int n_allowed;
+    const mv_logit_controls& c = a.c;
+    const int tid = threadIdx.x;
+    const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
+    const int v0 = (int)(chunk * LC_CHUNK);
+    const bool counted = c.history != nullptr, biased = c.bias_ids != nullptr;
+
+    // the logits are on their way while the words are gathered
+    f32x4_t x[LC_GROUPS], u[LC_GROUPS];
+#pragma unroll
+    for (int j = 0; j < LC_GROUPS; ++j) {
+        const int v = v0 + (j * LC_THREADS + tid) * 4, left = a.vocab - v;
+        x[j] = left > 0 ? lc_load<IN32>(a.logits, (int64_t)row * a.ld + v, left) : f32x4_t{0, 0, 0, 0};
+        u[j] = left > 0 && a.uncond ? lc_load<IN32>(a.uncond, (int64_t)row * a.ld + v, left) : f32x4_t{0, 0, 0, 0};
+    }
+    const uint32_t* mask = nullptr;
+    if (c.masks) {
+        const int index = c.mask_index ? c.mask_index[row] : (int)row;
+        if (index >= 0 && index < c.n_masks) mask = c.masks + (int64_t)index * c.ld_mask;
+    }
+
+    if (counted || biased) {
+#pragma unroll
+        for (int j = 0; j < LC_GROUPS; ++j) {
+            *(u32x4*)&count[(j * LC_THREADS + tid) * 4] = u32x4{0, 0, 0, 0};
+            if (biased) *(u32x4*)&entry[(j * LC_THREADS + tid) * 4] = u32x4{0, 0, 0, 0};
+        }
+        __syncthreads();
+        if (counted) {
+            const int len = c.history_len ? min(max(c.history_len[row], 0), c.history_cap) : c.history_cap;
+            const int prompt = c.prompt_len ? c.prompt_len[row] : 0;
+            const int32_t* h = c.history + (int64_t)row * c.ld_history;
+            for (int i = tid; i < len; i += LC_THREADS) {
+                const int id = h[i];
+                if (id >= v0 && id < a.vocab && id - v0 < LC_CHUNK) {
+                    if (i < prompt) atomicOr(&count[id - v0], 0x80000000u);
+                    else atomicAdd(&count[id - v0], 1u);
+                }
+            }
+        }
+        if (biased) {
+            const int32_t* ids = c.bias_ids + (int64_t)row * c.ld_bias;
+            for (int i = tid; i < c.n_bias; i += LC_THREADS) {
+                const int id = ids[i];
+                if (id >= v0 && id < a.vocab && id - v0 < LC_CHUNK) atomicMax(&entry[id - v0], (uint32_t)i + 1u);
+            }
+        }
+        __syncthreads();
+    }
+
+    const float g = a.uncond ? c.guidance[row] : 0.f;
+    const float rho = c.repetition ? c.repetition[row] : 1.f, pres = c.presence ? c.presence[row] : 0.f, freq = c.frequency ? c.frequency[row] : 0.f;
+#pragma unroll
+    for (int j = 0; j < LC_GROUPS; ++j) {
+        const int k = (j * LC_THREADS + tid) * 4, v = v0 + k, left = a.vocab - v;
+        if (left <= 0) break;
+        if (a.uncond) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (x[j][i] != -INFINITY) x[j][i] = g * x[j][i] + (1.f - g) * u[j][i];
+        }
+        if (counted) {
+            const u32x4 n4 = *(const u32x4*)&count[k];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (n4[i] == 0) continue;
+                x[j][i] = x[j][i] > 0.f ? x[j][i] / rho : x[j][i] * rho;
+                const uint32_t n = n4[i] & 0x7FFFFFFFu;
+                if (n) x[j][i] -= (float)n * freq + pres;
+            }
+        }
+        if (biased) {
+            const u32x4 e4 = *(const u32x4*)&entry[k];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e4[i]) x[j][i] += c.bias[(int64_t)row * c.ld_bias + e4[i] - 1];
+        }
+        if (mask) {
+            const uint32_t bits = mask[v >> 5] >> (v & 31);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!((bits >> i) & 1)) x[j][i] = -INFINITY;
+        }
+        const int64_t at = (int64_t)row * a.ld_out + v;
+        if (OUT32) {
+            float* o = (float*)a.out + at;
+            if (left >= 4) *(f32x4_any*)o = x[j];
+            else
+                for (int i = 0; i < left; ++i) o[i] = x[j][i];
+        } else {
+            bf16_t* o = (bf16_t*)a.out + at;
+            if (left >= 4) *(u32x2_any*)o = u32x2{pack_bf2(x[j][0], x[j][1]), pack_bf2(x[j][2], x[j][3])};
+            else
+                for (int i = 0; i < left; ++i) o[i] = f2bf(x[j][i]);
+        }
+    }
+
+    if (a.allowed != nullptr && chunk == 0) {  // the first chunk's workgroup counts the bits of the whole mask
+        int n = 0;
+        if (mask) {
+            for (int w = tid; w < (a.vocab + 31) / 32; w += LC_THREADS) {
+                const int left = a.vocab - w * 32;
+                n += __popc(left >= 32 ? mask[w] : mask[w] & ((1u << left) - 1u));
+            }
+        } else if (tid == 0) n = a.vocab;
+        if (tid == 0) n_allowed = 0;
+        __syncthreads();
+        if (n) atomicAdd(&n_allowed, n);
+        __syncthreads();
+        if (tid == 0) a.allowed[row] = n_allowed;
+    }
+}
+
+}  // namespace
+
+extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, int32_t dtype, const void* logits, const void* uncond, int64_t ld,
+                                    const mv_logit_controls* controls, int32_t out_dtype, void* out, int64_t ld_out, int32_t* allowed) {
+    if (rows < 0 || vocab < 1) return mv_fail(MV_ERR_INVALID, "logit_controls: bad shape rows=%d vocab=%d", rows, vocab);
+    if ((dtype != MV_BF16 && dtype != MV_F32) || (out_dtype != MV_BF16 && out_dtype != MV_F32))
+        return mv_fail(MV_ERR_INVALID, "logit_controls: dtype %d -> %d (MV_BF16 or MV_F32)", dtype, out_dtype);
+    if (ld < vocab || ld_out < vocab) return mv_fail(MV_ERR_INVALID, "logit_controls: a row stride (%lld, %lld) is below the vocabulary %d", (long long)ld, (long long)ld_out, vocab);
+    if (!controls) return mv_fail(MV_ERR_INVALID, "logit_controls: null argument");
+    ControlArgs a{*controls, logits, uncond, out, allowed, ld, ld_out, vocab, 0};
+    mv_logit_controls& c = a.c;
+    if (uncond && !c.guidance) return mv_fail(MV_ERR_INVALID, "logit_controls: uncond without guidance");
+    if (c.history_cap < 0 || c.n_bias < 0 || c.n_masks < 0) return mv_fail(MV_ERR_INVALID, "logit_controls: a negative count");
+    if (c.history && c.ld_history < c.history_cap) return mv_fail(MV_ERR_INVALID, "logit_controls: ld_history below history_cap");
+    if (!c.history && c.history_cap) return mv_fail(MV_ERR_INVALID, "logit_controls: history_cap without history");
+    if (!c.bias_ids != !c.bias || (!c.bias && c.n_bias)) return mv_fail(MV_ERR_INVALID, "logit_controls: bias_ids, bias and n_bias go together");
+    if (c.bias && c.ld_bias != 0 && c.ld_bias < c.n_bias) return mv_fail(MV_ERR_INVALID, "logit_controls: ld_bias is neither 0 nor n_bias or more");
+    if (!c.masks && (c.n_masks || c.mask_index)) return mv_fail(MV_ERR_INVALID, "logit_controls: n_masks or mask_index without masks");
+    if (c.masks && c.ld_mask < (vocab + 31LL) / 32) return mv_fail(MV_ERR_INVALID, "logit_controls: ld_mask below one bit per token");
+    if (c.masks && !c.mask_index && c.n_masks < rows) return mv_fail(MV_ERR_INVALID, "logit_controls: %d masks for %d rows and no mask_index", c.n_masks, rows);
+    if (rows == 0) return MV_OK;
+    if (!logits || !out) return mv_fail(MV_ERR_INVALID, "logit_controls: null argument");
+    const size_t ein = dtype == MV_F32 ? 4 : 2, eout = out_dtype == MV_F32 ? 4 : 2;
+    if (!op_aligned(logits, ein) || !op_aligned(uncond, ein) || !op_aligned(out, eout)) return mv_fail(MV_ERR_INVALID, "logit_controls: a buffer is not aligned to its element");
+    if (c.history_cap == 0 || (!c.repetition && !c.presence && !c.frequency)) c.history = nullptr;
+    if (c.n_bias == 0) c.bias_ids = nullptr;
+    a.chunks = (uint32_t)((vocab + (int64_t)LC_CHUNK - 1) / LC_CHUNK);
+    if ((int64_t)a.chunks * rows > 0x7FFFFFFF) return mv_fail(MV_ERR_INVALID, "logit_controls: rows=%d vocab=%d is too large", rows, vocab);
+    OpDevice dev((hipStream_t)stream, out);
+    LC_TRY(dev.status());
+    const dim3 grid(a.chunks * (uint32_t)rows), block(LC_THREADS);
+    if (dtype == MV_F32 && out_dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<true, true>), grid, block, 0, (hipStream_t)stream, a);
+    else if (dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<true, false>), grid, block, 0, (hipStream_t)stream, a);
+    else if (out_dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<false, true>), grid, block, 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((logit_controls_kernel<false, false>), grid, block, 0, (hipStream_t)stream, a);
+    LC_TRY(hipGetLastError());
+    return MV_OK;
+}

@@ -1,0 +1,58 @@
+// Host-side helpers of the stand-alone operators (mxfp4.hip, logits.hip): error reporting and the device a call works on.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "../../include/metavoice_hip.h"
+
+int mv_fail(int code, const char* fmt, ...);
+
+// Kernels are launched on the device that owns the stream; the null stream names no device, so there the device of `p` (a buffer of the call)
+// decides.  The calling thread's current device is restored.  With one device in the process nothing is asked.
+class OpDevice {
+  public:
+    OpDevice(hipStream_t s, const void* p) {
+        static const int count = [] {
+            int n = 0;
+            return hipGetDeviceCount(&n) == hipSuccess ? n : 0;
+        }();
+        if (count <= 1) return;
+        int want = -1, cur = -1;
+        if ((status_ = hipGetDevice(&cur)) != hipSuccess) return;
+        if (s == nullptr || s == hipStreamLegacy || s == hipStreamPerThread) {
+            hipPointerAttribute_t attr;
+            if ((status_ = hipPointerGetAttributes(&attr, p)) != hipSuccess) return;
+            want = attr.device;
+        } else {
+            hipDevice_t d = -1;
+            if ((status_ = hipStreamGetDevice(s, &d)) != hipSuccess) return;
+            want = d;
+        }
+        if (want != cur && want >= 0) {
+            status_ = hipSetDevice(want);
+            if (status_ == hipSuccess) prev_ = cur;
+        }
+    }
+    ~OpDevice() {
+        if (prev_ >= 0) (void)hipSetDevice(prev_);
+    }
+    OpDevice(const OpDevice&) = delete;
+    OpDevice& operator=(const OpDevice&) = delete;
+    hipError_t status() const { return status_; }
+
+  private:
+    int prev_ = -1;
+    hipError_t status_ = hipSuccess;
+};
+
+inline bool op_aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
+// n / d for 0 <= n < 2^31 by a multiply and a shift
+struct FastDiv {
+    uint32_t mul = 0, shift = 0, d = 1;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div) {
+        while ((1ull << shift) < div) ++shift;
+        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - div)) / div + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};

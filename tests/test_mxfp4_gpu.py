@@ -1,0 +1,289 @@
+"""MXFP4 quantiser and products (mv_op_quantize_mxfp4, mv_op_linear_mxfp4, mv_op_gemm_mxfp4) on the GPU against oracle/mxfp4.py (64 bits).
+
+The quantiser and its values are exact.  A product's tolerance counts roundings: a term passes the additions inside one matrix instruction (at most
+128), one per instruction along K (at most K / 32) and one per partial sum that is joined (at most 64), each off by at most 2^-23 of the magnitudes
+summed; the output's own rounding is half a step (2^-8 bf16, 2^-24 fp32)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import load_pkg
+from oracle import mxfp4 as o_mx
+
+pytestmark = pytest.mark.gpu
+
+N = load_pkg("_native")
+CODE = {torch.bfloat16: 0, torch.float32: 1}
+
+
+def ptr(t):
+    return C.c_void_p(t.data_ptr()) if t is not None else None
+
+
+def stream():
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def bits64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def hip_quantize(w, k=None, deq=True):
+    n, ld = w.shape[0], w.stride(0)
+    k = w.shape[1] if k is None else k
+    nb = o_mx.blocks(k)
+    codes = torch.full((n + 1, 16 * nb), 0x5A, dtype=torch.uint8, device="cuda")  # one row more than is quantised: it stays as it is
+    scales = torch.full((n + 1, nb), 0x5A, dtype=torch.uint8, device="cuda")
+    d = torch.full((n + 1, k), 7.0, dtype=torch.bfloat16, device="cuda") if deq else None
+    N.check(N.lib().mv_op_quantize_mxfp4(stream(), n, k, CODE[w.dtype], ptr(w), ld, ptr(codes), ptr(scales), ptr(d)))
+    torch.cuda.synchronize()
+    assert bool((codes[n] == 0x5A).all()) and bool((scales[n] == 0x5A).all()) and (d is None or bool((d[n] == 7).all()))
+    return codes[:n], scales[:n], None if d is None else d[:n]
+
+
+def check_quantised(w, codes, scales, deq):
+    c, s = o_mx.quantize(bits64(w))
+    assert np.array_equal(scales.cpu().numpy(), s)
+    assert np.array_equal(codes.cpu().numpy(), c)
+    if deq is not None:
+        assert np.array_equal(bits64(deq), o_mx.values(c, s, w.shape[1]), equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,k", [(1, 1), (1, 31), (3, 32), (5, 33), (2, 64), (7, 100), (33, 257), (64, 2048), (300, 1111)])
+@pytest.mark.parametrize("pad", [0, 1, 8])
+def test_quantiser_is_exact(n, k, dtype, pad):
+    g = torch.Generator().manual_seed(n * 1000 + k)
+    w = (torch.randn(n, k + pad, generator=g) * torch.exp(4 * torch.randn(n, 1, generator=g))).to(dtype)
+    w[0, 0] = 0
+    w[n - 1, max(0, k - 32):] = 0  # a block of zeros
+    w = w.cuda()[:, :k]
+    check_quantised(w, *hip_quantize(w))
+    check_quantised(w, *hip_quantize(w, deq=False))
+
+
+def test_quantiser_over_all_bf16_numbers_and_ties():
+    """Every bf16 bit pattern against itself and a large neighbour; and every tie of the grid at every block exponent."""
+    every = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    w = every.view(-1, 32).cuda()  # blocks of one exponent; some hold infinities and NaN
+    check_quantised(w, *hip_quantize(w))
+    fine = torch.where(torch.isfinite(every.float()), every, torch.zeros_like(every)).view(-1, 1).expand(-1, 32).clone()
+    fine[:, 1:] = 0
+    fine = fine.cuda()
+    check_quantised(fine, *hip_quantize(fine))
+    tie = torch.tensor([0, .25, .5, .75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, 7]).repeat(2)
+    tie[16:] *= -1
+    t32 = torch.ldexp(tie.double().view(1, 32), torch.arange(-126, 125, dtype=torch.float64).view(-1, 1)).float()
+    t32 = torch.cat([t32, torch.nextafter(t32, torch.zeros_like(t32)), torch.nextafter(t32, t32 * 2)]).cuda()
+    check_quantised(t32, *hip_quantize(t32))
+
+
+def test_quantiser_marks_blocks_that_are_not_finite():
+    w = torch.randn(4, 96)
+    w[0, 5], w[1, 40], w[2, 95], w[3, 0] = float("inf"), float("-inf"), float("nan"), 3.0e38
+    for dt in (torch.bfloat16, torch.float32):
+        d = w.to(dt).cuda()
+        codes, scales, deq = hip_quantize(d)
+        check_quantised(d, codes, scales, deq)
+        assert (scales.cpu() == 255).nonzero().tolist() == [[0, 0], [1, 1], [2, 2]]
+
+
+def test_quantiser_in_place():
+    w = (torch.randn(40, 256) * 0.1).bfloat16().cuda()
+    c, s = o_mx.quantize(bits64(w))
+    codes, scales = torch.zeros(40, 128, dtype=torch.uint8, device="cuda"), torch.zeros(40, 8, dtype=torch.uint8, device="cuda")
+    N.check(N.lib().mv_op_quantize_mxfp4(stream(), 40, 256, 0, ptr(w), 256, ptr(codes), ptr(scales), ptr(w)))
+    torch.cuda.synchronize()
+    assert np.array_equal(bits64(w), o_mx.values(c, s, 256))
+
+
+def make(g, n, k, spread=1.0):
+    codes, scales = o_mx.quantize((torch.randn(n, k, generator=g) * torch.exp(spread * torch.randn(n, 1, generator=g))).double().numpy())
+    return codes, scales
+
+
+def dev(a):
+    return torch.from_numpy(a).cuda()
+
+
+def product(kind, x, w, w2=None, bias=None, bias2=None, residual=None, out_dtype=torch.bfloat16, k=None, in_place=False):
+    """x: bf16 tensor, or (codes, scales); returns the output and asserts that the row behind it is left alone."""
+    m = (x if kind == "linear" else x[0]).shape[0]
+    n = w[0].shape[0]
+    out = torch.full((m + 1, n), 7.0, dtype=out_dtype, device="cuda")
+    if in_place:
+        out[:m] = residual
+        residual = out
+    act = (ptr(x), x.stride(0)) if kind == "linear" else (ptr(x[0]), ptr(x[1]))
+    w2 = w2 or (None, None)
+    fn = N.lib().mv_op_linear_mxfp4 if kind == "linear" else N.lib().mv_op_gemm_mxfp4
+    N.check(fn(stream(), m, n, k, *act, ptr(w[0]), ptr(w[1]), ptr(w2[0]), ptr(w2[1]), ptr(bias), ptr(bias2), ptr(residual), CODE[out_dtype], ptr(out)))
+    torch.cuda.synchronize()
+    assert bool((out[m] == 7).all())
+    return out[:m]
+
+
+def within(got, want, size, k, dtype):
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    tol = (128 + k / 32 + 64) * 2.0 ** -23 * size + half * np.abs(want) + 1e-37
+    got = bits64(got)
+    assert got.shape == want.shape
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), f"{bad.sum()} of {bad.size} off, first at {np.argwhere(bad)[0]}: {got[bad][0]} against {want[bad][0]}, {np.abs(got - want)[bad][0] / tol[bad][0]:.2f} tolerances"
+
+
+SHAPES = [(1, 1, 1), (1, 16, 32), (2, 2562, 2048), (3, 17, 33), (5, 40, 96), (16, 64, 128), (17, 100, 127), (33, 48, 640), (48, 320, 4096), (64, 129, 1000),
+          (65, 260, 512), (100, 1000, 736), (128, 128, 256), (130, 257, 511), (200, 512, 1024), (257, 300, 2080), (512, 520, 288), (300, 1030, 31)]
+
+
+def case(kind, m, n, k, gated, bias, residual, dtype, pad=0):
+    g = torch.Generator().manual_seed(m * 7 + n * 3 + k)
+    if kind == "linear":
+        x = torch.randn(m, k + pad, generator=g).bfloat16().cuda()[:, :k]
+        x64 = bits64(x)
+    else:
+        xc = make(g, m, k)
+        x, x64 = (dev(xc[0]), dev(xc[1])), o_mx.values(*xc, k)
+    w, w2 = make(g, n, k), make(g, n, k) if gated else None
+    b = torch.randn(n, generator=g).bfloat16() if bias else None
+    b2 = torch.randn(n, generator=g).bfloat16() if bias and gated else None
+    res = torch.randn(m, n, generator=g).to(dtype) if residual else None
+    f = lambda t: None if t is None else t.double().numpy()  # noqa: E731
+    want, size = o_mx.product(x64, o_mx.values(*w, k), None if w2 is None else o_mx.values(*w2, k), f(b), f(b2), f(res))
+    up = lambda t: None if t is None else t.cuda()  # noqa: E731
+    args = dict(x=x, w=(dev(w[0]), dev(w[1])), w2=None if w2 is None else (dev(w2[0]), dev(w2[1])), bias=up(b), bias2=up(b2), residual=up(res), out_dtype=dtype, k=k)
+    return args, want, size
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+def test_product(kind, m, n, k):
+    for gated, bias, residual, dtype in ((False, False, False, torch.bfloat16), (False, True, True, torch.float32), (True, False, False, torch.bfloat16),
+                                         (True, True, True, torch.bfloat16)):
+        args, want, size = case(kind, m, n, k, gated, bias, residual, dtype)
+        within(product(kind, **args), want, size, k, dtype)
+
+
+@pytest.mark.parametrize("pad", [1, 3, 8])
+@pytest.mark.parametrize("m,n,k", [(2, 100, 640), (20, 64, 333), (150, 200, 1024), (300, 300, 500)])
+def test_linear_of_strided_rows(m, n, k, pad):
+    args, want, size = case("linear", m, n, k, False, True, False, torch.float32, pad)
+    within(product("linear", **args), want, size, k, torch.float32)
+
+
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_residual_in_place(kind, m):
+    args, want, size = case(kind, m, 272, 512, False, False, True, torch.bfloat16)
+    within(product(kind, in_place=True, **args), want, size, 512, torch.bfloat16)
+
+
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_extreme_and_nan_scales(kind, m):
+    """The smallest block exponents (values below the smallest normal bf16) still count, the largest do not overflow on the way, and a NaN block
+    reaches the outputs of its own weight row or its own x row alone."""
+    n, k = 80, 256
+    g = torch.Generator().manual_seed(5)
+    args, _, _ = case(kind, m, n, k, False, False, False, torch.float32)
+    wc, ws = make(g, n, k, 0.0)
+    ws[0], ws[1], ws[2] = 0, 1, 250
+    if kind == "linear":
+        x = torch.randn(m, k, generator=g)
+        x64 = (x * 2.0 ** 100).bfloat16().double().numpy()
+        args["x"] = torch.from_numpy(x64).bfloat16().cuda()
+        ws[2] = 140
+    else:
+        xc, xs = make(g, m, k, 0.0)
+        xs[:, 1] = 227
+        ws[2] = 20
+        args["x"], x64 = (dev(xc), dev(xs)), o_mx.values(xc, xs, k)
+    args["w"] = (dev(wc), dev(ws))
+    want, size = o_mx.product(x64, o_mx.values(wc, ws, k))
+    within(product(kind, **args), want, size, k, torch.float32)
+    ws[7, 3] = 255
+    args["w"] = (dev(wc), dev(ws))
+    got = product(kind, **args)
+    assert bool(torch.isnan(got[:, 7]).all()) and not bool(torch.isnan(torch.cat([got[:, :7], got[:, 8:]], 1)).any())
+    if kind == "gemm":
+        ws[7, 3], xs[m - 1, 0] = 127, 255
+        args["w"], args["x"] = (dev(wc), dev(ws)), (dev(xc), dev(xs))
+        got = product(kind, **args)
+        assert bool(torch.isnan(got[m - 1]).all()) and not bool(torch.isnan(got[: m - 1]).any())
+
+
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+def test_empty_calls_touch_nothing(kind):
+    args, _, _ = case(kind, 4, 16, 64, False, False, False, torch.float32)
+    out = torch.full((4, 16), 7.0, device="cuda")
+    act = (ptr(args["x"]), 64) if kind == "linear" else (ptr(args["x"][0]), ptr(args["x"][1]))
+    fn = N.lib().mv_op_linear_mxfp4 if kind == "linear" else N.lib().mv_op_gemm_mxfp4
+    for m, n in ((0, 16), (4, 0)):
+        N.check(fn(stream(), m, n, 64, *act, ptr(args["w"][0]), ptr(args["w"][1]), None, None, None, None, None, 1, ptr(out)))
+    N.check(N.lib().mv_op_quantize_mxfp4(stream(), 0, 64, 1, ptr(out), 64, None, None, None))
+    torch.cuda.synchronize()
+    assert bool((out == 7).all())
+
+
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_results_do_not_depend_on_the_batch_or_the_run(m):
+    """A row's result has the same bits on every run."""
+    for kind in ("linear", "gemm"):
+        args, _, _ = case(kind, m, 400, 2048, True, True, True, torch.bfloat16)
+        first = product(kind, **args)
+        for _ in range(5):
+            assert torch.equal(product(kind, **args), first)
+
+
+def test_products_on_two_streams_and_in_a_graph():
+    """Calls share nothing: two streams at once, and a captured chain (quantise -> 4-bit product -> bf16 product) replayed on new inputs between
+    eager calls."""
+    m, n, k = 48, 640, 512
+    g = torch.Generator().manual_seed(11)
+    w, wb = tuple(map(dev, make(g, n, k))), tuple(map(dev, make(g, k, n)))
+    x = torch.randn(m, k, generator=g).bfloat16().cuda()
+    bufs = lambda: (torch.zeros(m, k // 2, dtype=torch.uint8, device="cuda"), torch.zeros(m, k // 32, dtype=torch.uint8, device="cuda"),  # noqa: E731
+                    torch.zeros(m, n, dtype=torch.bfloat16, device="cuda"), torch.zeros(m, k, dtype=torch.float32, device="cuda"))
+
+    def chain(src, b):
+        lib, s = N.lib(), stream()
+        N.check(lib.mv_op_quantize_mxfp4(s, m, k, 0, ptr(src), k, ptr(b[0]), ptr(b[1]), None))
+        N.check(lib.mv_op_gemm_mxfp4(s, m, n, k, ptr(b[0]), ptr(b[1]), ptr(w[0]), ptr(w[1]), None, None, None, None, None, 0, ptr(b[2])))
+        N.check(lib.mv_op_linear_mxfp4(s, m, k, n, ptr(b[2]), n, ptr(wb[0]), ptr(wb[1]), None, None, None, None, None, 1, ptr(b[3])))
+        return b[3]
+
+    want = chain(x, bufs()).clone()
+    c64, s64 = o_mx.quantize(bits64(x))
+    y, size = o_mx.product(o_mx.values(c64, s64, k), o_mx.values(w[0].cpu().numpy(), w[1].cpu().numpy(), k))
+    mid = bufs()
+    chain(x, mid)
+    within(mid[2], y, size, k, torch.bfloat16)
+    z, zsize = o_mx.product(bits64(mid[2]), o_mx.values(wb[0].cpu().numpy(), wb[1].cpu().numpy(), n))
+    within(mid[3], z, zsize, n, torch.float32)
+
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    b1, b2 = bufs(), bufs()
+    torch.cuda.synchronize()
+    for _ in range(8):
+        with torch.cuda.stream(s1):
+            chain(x, b1)
+        with torch.cuda.stream(s2):
+            chain(x, b2)
+    torch.cuda.synchronize()
+    assert torch.equal(b1[3], want) and torch.equal(b2[3], want)
+
+    static, gb = x.clone(), bufs()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        chain(static, gb)
+    for i in range(4):
+        new = torch.randn(m, k, generator=g).bfloat16().cuda()
+        static.copy_(new)
+        graph.replay()
+        eager = chain(new, bufs())
+        torch.cuda.synchronize()
+        assert torch.equal(gb[3], eager)
