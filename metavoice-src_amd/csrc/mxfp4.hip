@@ -12,12 +12,16 @@
 #include "op_common.h"
 
 #include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <type_traits>
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));  // 16 bytes at the alignment of a bf16 element
+typedef u32x4 u32x4_any __attribute__((aligned(2)));    // 16 bytes at the alignment of a bf16 element
+typedef f32x4_t f32x4_any __attribute__((aligned(4)));  // and of a float
 
 #define MX_TRY(expr)                                                                                                               \
     do {                                                                                                                           \
@@ -116,6 +120,7 @@ struct MxArgs {
     int64_t ldx;
     int32_t M, N, K, nb, out_f32;
     uint32_t tiles_n;
+    int32_t x_direct, s_direct;  // rows of x and of scales are aligned to 4 bytes
 };
 
 // y = x . w + bias (gated: silu(y) * (x . w2 + bias2)) + residual, in fp32, rounded once
@@ -132,6 +137,47 @@ __device__ __forceinline__ void mx_store(const MxArgs& a, int m, int n, float v,
     } else {
         if (a.res) v += bf2f(((const bf16_t*)a.res)[at]);
         ((bf16_t*)a.out)[at] = f2bf(v);
+    }
+}
+
+// mx_store for 8 consecutive columns
+__device__ __forceinline__ void mx_store8(const MxArgs& a, int m, int n, float (&v)[8], float (&v2)[8]) {
+    if (n + 8 > a.N) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (n + e < a.N) mx_store(a, m, n + e, v[e], v2[e]);
+        return;
+    }
+    if (a.bias) {
+        const u32x4 b = *(const u32x4_any*)(a.bias + n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += e & 1 ? bf_hi(b[e >> 1]) : bf_lo(b[e >> 1]);
+    }
+    if (a.w2) {
+        if (a.bias2) {
+            const u32x4 b = *(const u32x4_any*)(a.bias2 + n);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v2[e] += e & 1 ? bf_hi(b[e >> 1]) : bf_lo(b[e >> 1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.0f + __expf(-v[e])) * v2[e];
+    }
+    const int64_t at = (int64_t)m * a.N + n;
+    if (a.out_f32) {
+        if (a.res) {
+            const f32x4_any lo = *(const f32x4_any*)((const float*)a.res + at), hi = *(const f32x4_any*)((const float*)a.res + at + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[4 + e] += hi[e]; }
+        }
+        *(f32x4_any*)((float*)a.out + at) = f32x4_t{v[0], v[1], v[2], v[3]};
+        *(f32x4_any*)((float*)a.out + at + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+    } else {
+        if (a.res) {
+            const u32x4 q = *(const u32x4_any*)((const bf16_t*)a.res + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += e & 1 ? bf_hi(q[e >> 1]) : bf_lo(q[e >> 1]);
+        }
+        *(u32x4_any*)((bf16_t*)a.out + at) = u32x4{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])};
     }
 }
 
@@ -156,99 +202,584 @@ __device__ __forceinline__ bf16x8_t mx_widen(uint32_t q, float scale) {
 
 #define MX_WAVES 8
 
-// One workgroup: 16 weight rows against 16 rows of x; the waves take the 128-column steps of K in turn and their sums meet in LDS, in wave order.
-// Lane (r = lane & 15, g = lane >> 4) holds block 4 step + g of weight row r and of x row r.  The weights are the first operand of the matrix
-// instruction, so a lane ends with 4 consecutive output columns of one row.
-template <bool X4, bool GATED>
-__global__ void __launch_bounds__(64 * MX_WAVES) mx_rows_kernel(const MxArgs a) {
-    __shared__ f32x4_t part[GATED ? 2 : 1][MX_WAVES][64];
+// Few rows: one workgroup computes 16 MT rows of x against 16 NT weight rows; its waves take the 128-column steps of K in turn, each straight from memory
+// to registers, and their sums meet in LDS, in wave order.  Lane (r = lane & 15, g = lane >> 4) holds block 4 step + g of weight row r and of x row
+// r: the weights are the first operand of the matrix instruction, so a lane ends with 4 consecutive output columns of one row.  Bound by what a CU reads
+// (about 30 bytes per nanosecond of x and weights), or by latency when the matrix is small.
+template <bool X4, bool GATED, int MT, int NT>
+__global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs a) {
+    constexpr int MATS = GATED ? 2 : 1, XW = X4 ? 1 : 4;  // 16-byte pieces of an x row per step
+    extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [wave][matrix, weight tile, x tile][lane]
+    constexpr int TILES = MATS * NT * MT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const uint32_t tm = blockIdx.x / a.tiles_n, tn = blockIdx.x - tm * a.tiles_n;
-    const int m = (int)tm * 16 + r, n = (int)tn * 16 + r;
-    const bool has_m = m < a.M, has_n = n < a.N;
-    f32x4_t acc[GATED ? 2 : 1];
-    acc[0] = f32x4_t{0, 0, 0, 0};
-    if (GATED) acc[GATED ? 1 : 0] = f32x4_t{0, 0, 0, 0};
+    const int m0 = (int)tm * 16 * MT, n0 = (int)tn * 16 * NT;
+    f32x4_t acc[MATS][NT][MT];
+#pragma unroll
+    for (int i = 0; i < MATS; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[i][n][m] = f32x4_t{0, 0, 0, 0};
     for (int b0 = wave * 4; b0 < a.nb; b0 += MX_WAVES * 4) {
         const int b = b0 + g;
         const bool in_k = b < a.nb;
-        u32x4 wq[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
-        uint32_t wsc[2] = {127u, 127u};
-        if (in_k && has_n) {
-            const int64_t at = (int64_t)n * a.nb + b;
-            wq[0] = *(const u32x4*)(a.w + at * 16);
-            wsc[0] = a.ws[at];
-            if (GATED) {
-                wq[1] = *(const u32x4*)(a.w2 + at * 16);
-                wsc[1] = a.ws2[at];
+        u32x4 wq[MATS][NT], xq[MT][XW];
+        uint32_t wsc[MATS][NT], xsc[MT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = n0 + n * 16 + r;
+            const bool in = in_k && row < a.N;
+            const int64_t at = (int64_t)row * a.nb + b;
+#pragma unroll
+            for (int i = 0; i < MATS; ++i) {
+                wq[i][n] = u32x4{0u, 0u, 0u, 0u};
+                wsc[i][n] = 127u;
+                if (in) {
+                    wq[i][n] = *(const u32x4*)((i ? a.w2 : a.w) + at * 16);
+                    wsc[i][n] = (i ? a.ws2 : a.ws)[at];
+                }
             }
         }
-        if (X4) {
-            u32x4 xq = {0u, 0u, 0u, 0u};
-            uint32_t xsc = 127u;
-            if (in_k && has_m) {
-                const int64_t at = (int64_t)m * a.nb + b;
-                xq = *(const u32x4*)((const unsigned char*)a.x + at * 16);
-                xsc = a.xs[at];
-            }
-            const i32x8_t xv = {(int)xq[0], (int)xq[1], (int)xq[2], (int)xq[3], 0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < (GATED ? 2 : 1); ++i) {
-                const i32x8_t wv = {(int)wq[i][0], (int)wq[i][1], (int)wq[i][2], (int)wq[i][3], 0, 0, 0, 0};
-                acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i], 4, 4, 0, (int)wsc[i], 0, (int)xsc);
-            }
-        } else {
+        for (int m = 0; m < MT; ++m) {
+            const int row = m0 + m * 16 + r;
+            const bool in = in_k && row < a.M;
+            xsc[m] = 127u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 xv = {0u, 0u, 0u, 0u};
-                if (in_k && has_m) xv = mx_load_x8((const bf16_t*)a.x + (int64_t)m * a.ldx, b * 32 + j * 8, a.K);
+            for (int j = 0; j < XW; ++j) xq[m][j] = u32x4{0u, 0u, 0u, 0u};
+            if (in) {
+                if (X4) {
+                    const int64_t at = (int64_t)row * a.nb + b;
+                    xq[m][0] = *(const u32x4*)((const unsigned char*)a.x + at * 16);
+                    xsc[m] = a.xs[at];
+                } else {
+                    const bf16_t* p = (const bf16_t*)a.x + (int64_t)row * a.ldx;
+                    if (b * 32 + 32 <= a.K) {
 #pragma unroll
-                for (int i = 0; i < (GATED ? 2 : 1); ++i)
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_widen(wq[i][j], __uint_as_float(wsc[i] << 23)), __builtin_bit_cast(bf16x8_t, xv), acc[i], 0, 0, 0);
+                        for (int j = 0; j < XW; ++j) xq[m][j] = *(const u32x4_any*)(p + b * 32 + j * 8);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < XW; ++j) xq[m][j] = mx_load_x8(p, b * 32 + j * 8, a.K);
+                    }
+                }
             }
         }
+#pragma unroll
+        for (int i = 0; i < MATS; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const u32x4 w = wq[i][n];
+                if (X4) {
+                    const i32x8_t wv = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const u32x4 x = xq[m][0];
+                        const i32x8_t xv = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+                        acc[i][n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i][n][m], 4, 4, 0, (int)wsc[i][n], 0, (int)xsc[m]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < XW; ++j) {
+                        const bf16x8_t wv = mx_widen(w[j], __uint_as_float(wsc[i][n] << 23));
+#pragma unroll
+                        for (int m = 0; m < MT; ++m)
+                            acc[i][n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, xq[m][j]), acc[i][n][m], 0, 0, 0);
+                    }
+                }
+            }
     }
 #pragma unroll
-    for (int i = 0; i < (GATED ? 2 : 1); ++i) part[i][wave][lane] = acc[i];
+    for (int i = 0; i < MATS; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) part[(wave * TILES + (i * NT + n) * MT + m) * 64 + lane] = acc[i][n][m];
     __syncthreads();
-    if (threadIdx.x >= 256) return;
-    const int ln = threadIdx.x >> 2, c = threadIdx.x & 3;  // lane and register of the output element
-    float v = 0.f, v2 = 0.f;
+    // one output per thread and turn: neighbouring threads take neighbouring columns of a row
+    const float* sums = (const float*)part;
+    for (int o = threadIdx.x; o < MT * NT * 256; o += 64 * MX_WAVES) {
+        const int c = o % (16 * NT), row = o / (16 * NT);  // column and row in the workgroup's tile
+        const int at = (((c >> 4) * MT + (row >> 4)) * 64 + (((c & 15) >> 2) << 4) + (row & 15)) * 4 + (c & 3);
+        float v = 0.f, v2 = 0.f;
 #pragma unroll
-    for (int w = 0; w < MX_WAVES; ++w) {
-        v += part[0][w][ln][c];
-        if (GATED) v2 += part[GATED ? 1 : 0][w][ln][c];
+        for (int w = 0; w < MX_WAVES; ++w) {
+            v += sums[w * TILES * 256 + at];
+            if (GATED) v2 += sums[w * TILES * 256 + NT * MT * 256 + at];
+        }
+        if (m0 + row < a.M && n0 + c < a.N) mx_store(a, m0 + row, n0 + c, v, v2);
     }
-    const int om = (int)tm * 16 + (ln & 15), on = (int)tn * 16 + (ln >> 4) * 4 + c;
-    if (om < a.M && on < a.N) mx_store(a, om, on, v, v2);
 }
 
-hipError_t launch_products(hipStream_t s, MxArgs a, bool x4) {
-    a.tiles_n = (uint32_t)((a.N + 15) / 16);
-    const int64_t rows_per_launch = std::max<int64_t>(1, 0x7FFFFFFF / (int64_t)a.tiles_n / 16) * 16;  // a grid is below 2^31 workgroups
+// ---- large products -----------------------------------------------------------------------------------------------------------------------
+// One workgroup computes BM rows of x against BN weight rows, a wave 32 TX x 32 TW of them on 32x32 matrix instructions with the weights as the first
+// operand (a lane ends with 4 consecutive output columns of one row).  K advances in stages: 64 bf16 (128 bytes) or 128 codes (64 bytes) of a row.
+// Lane (r = lane & 31, h = lane >> 5) takes 16-byte chunk STEPS h + t of its row at step t.  With codes its steps are consecutive blocks: their scales
+// lie side by side and byte t of one register serves step t.  With bf16 its 4 steps are one block of its weight row: one 16-byte read of codes that it
+// widens 8 at a time.
+// Stages go from memory to LDS without registers, NBUF of them in LDS: the transfers run NBUF - 1 stages ahead, since one from another XCD's share of
+// memory takes longer than a stage.  The one barrier per stage stands before its last step, whose products cover its wait and the first reads of the
+// next stage; the reads of step t + 1 are covered by the products of step t.
+// Scales come 16 blocks of a row at a time, a group ahead, two groups in LDS (a few bytes per row and stage would touch as many cache lines as the
+// codes do).
+// LDS has 64 banks and serves 16 lanes of a 16-byte read at a time: chunk c of a row lies at c ^ (row / (rows per 256 bytes)), so 16 rows
+// spread over all banks.  A transfer writes LDS in lane order: the permutation is applied to the lane's address in memory.
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef const __attribute__((address_space(1))) void* glb_ptr_t;
+typedef u32x4 u32x4_byte __attribute__((aligned(1)));
+
+template <bool X4, int KS, int WN, int WM, int TW, int TX>
+struct Tile {
+    static constexpr int TEAM = WN * WM, WAVES = KS * TEAM, THREADS = 64 * WAVES;
+    static constexpr int BM = 32 * WM * TX, BN = 32 * WN * TW;       // rows of x and weight rows of a workgroup
+    static constexpr int XROW = 128, WROW = X4 ? 128 : 32;           // bytes of a row in a team's share of a stage
+    static constexpr int BLOCKS = X4 ? 8 : 2, STEPS = 4;             // blocks of 32 columns in it, and steps
+    static constexpr int GROUP = 16 / (BLOCKS * KS);                 // stages per group of scales
+    static constexpr int X = BM * XROW, W = BN * WROW, SHARE = X + W, STAGE = KS * SHARE;
+    static constexpr int SROWS = X4 ? BM + BN : BN, S = SROWS * 16;
+    // A group of scales has to be older than the transfers that a stage's wait leaves on their way: it is asked for AHEAD groups ahead, and lies in one
+    // of AHEAD + 1 places in turn, a short one at the end of a row in a place of its own.
+    static constexpr int fit(int bufs) { return bufs * STAGE + ((bufs + GROUP - 1) / GROUP + 2) * S; }
+    static constexpr int NBUF = fit(4) <= 160 * 1024 ? 4 : fit(3) <= 160 * 1024 ? 3 : 2;
+    static constexpr int AHEAD = (NBUF + GROUP - 1) / GROUP, RING = AHEAD + 1;
+    static constexpr int EPI = TEAM * 32 * (32 * TW + 4) * 4;        // the epilogue's tiles: 32 rows of a wave's columns each
+    static constexpr int JOIN = (KS - 1) * TEAM * TW * TX * 4096;    // the other teams' sums
+    static constexpr int MAIN = fit(NBUF), TAIL = EPI + JOIN, LDS = MAIN > TAIL ? MAIN : TAIL;
+    static constexpr int XI = X / 1024 / TEAM, WI = W / 1024 / TEAM;  // transfers of 1 KB per wave and stage
+    static_assert(XI * TEAM * 1024 == X && WI * TEAM * 1024 == W && LDS <= 160 * 1024, "whole transfers per wave");
+};
+
+template <int ROWB>
+__device__ __forceinline__ int mx_slot(int row, int c) { return c ^ ((row / (256 / ROWB)) & (ROWB / 16 - 1)); }
+
+template <bool X4, int KS, int WN, int WM, int TW, int TX, bool GATED>
+__global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxArgs a) {
+    typedef Tile<X4, KS, WN, WM, TW, TX> T;
+    constexpr int XCH = T::XROW / 16, WCH = T::WROW / 16, NBUF = T::NBUF;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave_of_all = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+    const int team = KS == 1 ? 0 : wave_of_all / T::TEAM, wave = KS == 1 ? wave_of_all : wave_of_all % T::TEAM;
+    const int wm = wave % WM, wn = wave / WM;
+    constexpr int NOUT = GATED ? T::BN / 2 : T::BN;  // output columns of a workgroup
+
+    // workgroups go round the 8 XCDs: each XCD takes a contiguous range of tiles, ordered in bands of 8 row tiles so that the tiles in flight on it
+    // share rows of x and of the weights in its L2
+    uint32_t id = blockIdx.x;
+    {
+        const uint32_t total = gridDim.x, q = total / 8, rem = total % 8, xcd = id % 8, k = id / 8;
+        id = xcd * q + min(xcd, rem) + k;
+    }
+    const uint32_t tiles_m = (uint32_t)((a.M + T::BM - 1) / T::BM);
+    const uint32_t band = id / (8 * a.tiles_n), in_band = id - band * 8 * a.tiles_n, rows_in = min(8u, tiles_m - band * 8);
+    const int m0 = (int)(band * 8 + in_band % rows_in) * T::BM, n0 = (int)(in_band / rows_in) * NOUT;
+
+    // row of the weights' LDS image -> matrix and weight row (gated: a wave's first half of columns from w, the second half the same columns of w2)
+    auto w_row = [&](int row, int& second) {
+        if (!GATED) { second = 0; return min(n0 + row, a.N - 1); }
+        second = (row / (16 * TW)) & 1;
+        return min(n0 + (row / (32 * TW)) * (16 * TW) + row % (16 * TW), a.N - 1);
+    };
+    const int64_t code_row = (int64_t)a.nb * 16, x_row = X4 ? code_row : a.ldx * 2;
+
+    // a lane's addresses in a stage: bytes from the workgroup's first row of x and first weight row
+    const unsigned char* const xbase = (const unsigned char*)a.x + (int64_t)m0 * x_row;
+    uint32_t gx[T::XI], gw[T::WI];
+    const unsigned char* wbase[T::WI];
+    static_assert(!GATED || (16 * TW) % (1024 / T::WROW) == 0, "a transfer reads one matrix");
+#pragma unroll
+    for (int i = 0; i < T::XI; ++i) {
+        const int row = (wave * T::XI + i) * (64 / XCH) + lane / XCH;
+        gx[i] = (uint32_t)min(row, a.M - 1 - m0) * (uint32_t)x_row + mx_slot<T::XROW>(row, lane % XCH) * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < T::WI; ++i) {
+        const int row = (wave * T::WI + i) * (64 / WCH) + lane / WCH;
+        int second;
+        gw[i] = (uint32_t)(w_row(row, second) - n0) * (uint32_t)code_row + mx_slot<T::WROW>(row, lane % WCH) * 16;
+        (void)w_row((wave * T::WI + i) * (64 / WCH), second);
+        wbase[i] = (second ? a.w2 : a.w) + (int64_t)n0 * code_row;
+    }
+    const int stages = (a.nb + KS * T::BLOCKS - 1) / (KS * T::BLOCKS);
+    const int direct = a.x_direct ? (X4 ? a.nb / (KS * 8) : a.K / (KS * 64)) : 0;  // the stages that are whole and aligned
+
+    const int share = team * T::SHARE;
+    auto transfer = [&](int st, int buf) {
+        const int v = st * KS + team;
+#pragma unroll
+        for (int i = 0; i < T::XI; ++i)
+            __builtin_amdgcn_global_load_lds((glb_ptr_t)(xbase + (int64_t)v * T::XROW + gx[i]), (lds_ptr_t)(lds + buf + share + (wave * T::XI + i) * 1024), 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < T::WI; ++i)
+            __builtin_amdgcn_global_load_lds((glb_ptr_t)(wbase[i] + (int64_t)v * T::WROW + gw[i]), (lds_ptr_t)(lds + buf + share + T::X + (wave * T::WI + i) * 1024), 16, 0, 0);
+    };
+    // the short stage at the end of a row, and rows of x that are not aligned: through registers, zeros past K
+    auto carry = [&](int st, int buf) {
+        const int v = st * KS + team, t = tid % (64 * T::TEAM);
+#pragma unroll 1
+        for (int i = t; i < T::X / 16; i += 64 * T::TEAM) {
+            const int row = i / XCH, c = mx_slot<T::XROW>(row, i % XCH), m = min(m0 + row, a.M - 1);
+            u32x4 q = {0u, 0u, 0u, 0u};
+            if (X4) {
+                if (v * T::BLOCKS + c < a.nb) q = *(const u32x4*)((const unsigned char*)a.x + m * x_row + (int64_t)(v * T::BLOCKS + c) * 16);
+            } else {
+                q = mx_load_x8((const bf16_t*)a.x + m * a.ldx, v * 64 + c * 8, a.K);
+            }
+            *(u32x4*)(lds + buf + share + i * 16) = q;
+        }
+#pragma unroll 1
+        for (int i = t; i < T::W / 16; i += 64 * T::TEAM) {
+            const int row = i / WCH, c = mx_slot<T::WROW>(row, i % WCH);
+            int second;
+            const int n = w_row(row, second);
+            u32x4 q = {0u, 0u, 0u, 0u};
+            if (v * T::BLOCKS + c < a.nb) q = *(const u32x4*)((second ? a.w2 : a.w) + n * code_row + (int64_t)(v * T::BLOCKS + c) * 16);
+            *(u32x4*)(lds + buf + share + T::X + i * 16) = q;
+        }
+    };
+    // scales of a group: 16 bytes of row t (with 4-bit x the rows of x come first) by transfer t / 64, wave after wave
+    constexpr int SBASE = NBUF * T::STAGE, SN = T::SROWS / 64, SI = (SN + T::WAVES - 1) / T::WAVES;
+    auto scale_row = [&](int row) {
+        if (X4 && row < T::BM) return a.xs + (int64_t)min(m0 + row, a.M - 1) * a.nb;
+        int second;
+        const int n = w_row(X4 ? row - T::BM : row, second);
+        return (second ? a.ws2 : a.ws) + (int64_t)n * a.nb;
+    };
+    const unsigned char* gs[SI];
+#pragma unroll
+    for (int i = 0; i < SI; ++i) gs[i] = scale_row(min(wave_of_all + i * T::WAVES, SN - 1) * 64 + lane);
+    const int whole_groups = a.nb / 16;
+    auto scale_at = [&](int group) { return SBASE + (group >= whole_groups ? T::RING : group % T::RING) * T::S; };
+    auto scales = [&](int group) {  // a whole, aligned group
+        const int to = scale_at(group);
+#pragma unroll
+        for (int i = 0; i < SI; ++i)
+            if (SN % T::WAVES == 0 || wave_of_all + i * T::WAVES < SN)
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)(gs[i] + group * 16), (lds_ptr_t)(lds + to + (wave_of_all + i * T::WAVES) * 1024), 16, 0, 0);
+    };
+    // whole groups of rows of scales that are not aligned to 4 bytes: through registers, asked for at one stage and put into LDS at the next
+    u32x4 sreg = {0u, 0u, 0u, 0u};
+    static_assert(T::SROWS <= T::THREADS, "a row of scales per thread");
+    auto scales_in = [&](int group) { sreg = *(const u32x4_byte*)(scale_row(min(tid, T::SROWS - 1)) + group * 16); };
+    auto scales_out = [&](int group) {
+        if (tid < T::SROWS) *(u32x4*)(lds + scale_at(group) + tid * 16) = sreg;
+    };
+    auto carry_scales = [&](int group) {  // at the start: a short group at the end of a row
+        const int b = group * 16, to = scale_at(group);
+#pragma unroll 1
+        for (int i = tid; i < T::SROWS * 4; i += T::THREADS) {
+            const unsigned char* p = scale_row(i >> 2);
+            uint32_t q = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) q |= (uint32_t)(b + (i & 3) * 4 + k < a.nb ? p[b + (i & 3) * 4 + k] : 127u) << (8 * k);
+            *(uint32_t*)(lds + to + i * 4) = q;
+        }
+    };
+
+    f32x16_t acc[TW][TX];
+#pragma unroll
+    for (int i = 0; i < TW; ++i)
+#pragma unroll
+        for (int j = 0; j < TX; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    u32x4 fx[2][TX], fw[2][TW];     // fragments of two steps; of bf16 stages the weights' are the stage's codes
+    uint32_t sx[2][TX], sw[2][TW];  // scales of a stage
+    int xat[T::STEPS], wat[X4 ? T::STEPS : 1];
+#pragma unroll
+    for (int t = 0; t < T::STEPS; ++t) {
+        xat[t] = share + (wm * 32 * TX + r) * T::XROW + mx_slot<T::XROW>(r, T::STEPS * h + t) * 16;
+        if (X4 || t == 0) wat[X4 ? t : 0] = share + T::X + (wn * 32 * TW + r) * T::WROW + mx_slot<T::WROW>(r, X4 ? T::STEPS * h + t : h) * 16;
+    }
+    auto read_x = [&](int buf, int t, u32x4 (&f)[TX]) {
+#pragma unroll
+        for (int j = 0; j < TX; ++j) f[j] = *(const u32x4*)(lds + buf + xat[t] + j * 32 * T::XROW);
+    };
+    auto read_w = [&](int buf, int t, u32x4 (&f)[TW]) {
+#pragma unroll
+        for (int i = 0; i < TW; ++i) f[i] = *(const u32x4*)(lds + buf + wat[X4 ? t : 0] + i * 32 * T::WROW);
+    };
+    auto read_s = [&](int st, uint32_t (&fsx)[TX], uint32_t (&fsw)[TW]) {
+        const unsigned char* buf = lds + scale_at(st / T::GROUP) + (st % T::GROUP * KS + team) * T::BLOCKS + (X4 ? h * 4 : h) + r * 16;
+        if (X4) {
+#pragma unroll
+            for (int j = 0; j < TX; ++j) fsx[j] = *(const uint32_t*)(buf + (wm * 32 * TX + j * 32) * 16);
+#pragma unroll
+            for (int i = 0; i < TW; ++i) fsw[i] = *(const uint32_t*)(buf + (T::BM + wn * 32 * TW + i * 32) * 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < TW; ++i) fsw[i] = buf[(wn * 32 * TW + i * 32) * 16];
+        }
+    };
+    // The products of a step.  They stay where they stand: left alone, the compiler carries them past the branches and reads of later steps, with all
+    // the registers that takes.
+    // The reads of the next step (`reads`) come behind the first products: the compiler waits for all reads on their way where it waits for one.
+    auto multiply = [&](auto step, const u32x4 (&x)[TX], const u32x4 (&w)[TW], const uint32_t (&csx)[TX], const uint32_t (&csw)[TW], auto reads) {
+        constexpr int t = decltype(step)::value;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < TW; ++i) {
+            if constexpr (X4) {
+                const i32x8_t wv = {(int)w[i][0], (int)w[i][1], (int)w[i][2], (int)w[i][3], 0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < TX; ++j) {
+                    const i32x8_t xv = {(int)x[j][0], (int)x[j][1], (int)x[j][2], (int)x[j][3], 0, 0, 0, 0};
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv, xv, acc[i][j], 4, 4, t, (int)csw[i], t, (int)csx[j]);
+                }
+            } else {
+                const bf16x8_t wv = mx_widen(w[i][t], __uint_as_float(csw[i] << 23));
+#pragma unroll
+                for (int j = 0; j < TX; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv, __builtin_bit_cast(bf16x8_t, x[j]), acc[i][j], 0, 0, 0);
+            }
+            if (i == 0) {
+#pragma unroll
+                for (int j = 0; j < TX; ++j) asm volatile("" : "+v"(acc[i][j]));
+                __builtin_amdgcn_sched_barrier(0);
+                reads();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int i = 1; i < TW; ++i)
+#pragma unroll
+            for (int j = 0; j < TX; ++j) asm volatile("" : "+v"(acc[i][j]));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+#pragma unroll
+    for (int i = 0; i < T::AHEAD; ++i)
+        if (a.s_direct && i < whole_groups) scales(i);
+#pragma unroll
+    for (int i = 0; i < NBUF; ++i) {
+        if (i < direct) transfer(i, i * T::STAGE);
+        else if (i < stages) carry(i, i * T::STAGE);
+    }
+    if (a.nb % 16) carry_scales(whole_groups);
+    if (!a.s_direct)
+        for (int i = 0; i < min(T::AHEAD, whole_groups); ++i) {
+            scales_in(i);
+            scales_out(i);
+        }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read_s(0, sx[0], sw[0]);
+    read_w(0, 0, fw[0]);
+    read_x(0, 0, fx[0]);
+
+    int cur = 0;  // byte offset of the stage's buffer
+    const auto wait_and_ask = [&](auto kind, int st) {
+        constexpr bool DIRECT = decltype(kind)::value;
+        if (!DIRECT && !a.s_direct && (st - 1) % T::GROUP == 0 && st > 0 && (st - 1) / T::GROUP + T::AHEAD < whole_groups) scales_out((st - 1) / T::GROUP + T::AHEAD);
+        // stage st + 1 must have arrived, NBUF - 2 later ones may be on their way (a request for scales among them only makes the wait longer)
+        if (st + NBUF - 1 < direct) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NBUF - 2) * (T::XI + T::WI)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        // and every wave has read all of stage st: its buffer is free
+        if (st + NBUF < direct) transfer(st + NBUF, cur);
+        else if (!DIRECT && st + NBUF < stages) carry(st + NBUF, cur);
+        if (st % T::GROUP == 0 && st / T::GROUP + T::AHEAD < whole_groups) {
+            if (DIRECT || a.s_direct) scales(st / T::GROUP + T::AHEAD);
+            else scales_in(st / T::GROUP + T::AHEAD);
+        }
+    };
+    // A stage, P its parity.  DIRECT: all that it asks for comes without registers.  (In one loop with the other kind, the compiler would let every read
+    // of LDS wait for all that are on their way.)
+    auto stage = [&](auto parity, auto kind, int st) {
+        constexpr int P = decltype(parity)::value;
+        const int next = cur + T::STAGE == NBUF * T::STAGE ? 0 : cur + T::STAGE;
+        multiply(std::integral_constant<int, 0>{}, fx[0], fw[X4 ? 0 : P], sx[P], sw[P], [&] {
+            read_x(cur, 1, fx[1]);
+            if (X4) read_w(cur, 1, fw[1]);
+        });
+        multiply(std::integral_constant<int, 1>{}, fx[1], fw[X4 ? 1 : P], sx[P], sw[P], [&] {
+            read_x(cur, 2, fx[0]);
+            if (X4) read_w(cur, 2, fw[0]);
+        });
+        multiply(std::integral_constant<int, 2>{}, fx[0], fw[X4 ? 0 : P], sx[P], sw[P], [&] {
+            read_x(cur, 3, fx[1]);
+            if (X4) read_w(cur, 3, fw[1]);
+        });
+        if (st + 1 < stages) wait_and_ask(kind, st);
+        multiply(std::integral_constant<int, 3>{}, fx[1], fw[X4 ? 1 : P], sx[P], sw[P], [&] {
+            if (st + 1 < stages) {
+                read_s(st + 1, sx[P ^ 1], sw[P ^ 1]);
+                read_w(next, 0, fw[X4 ? 0 : P ^ 1]);
+                read_x(next, 0, fx[0]);
+            }
+        });
+        cur = next;
+    };
+    const int easy = !a.s_direct ? 0 : direct == stages ? stages : max(0, direct - NBUF) & ~1;
+    int st = 0;
+#pragma unroll 1
+    for (; st < easy; st += 2) {
+        stage(std::integral_constant<int, 0>{}, std::true_type{}, st);
+        if (st + 1 < easy) stage(std::integral_constant<int, 1>{}, std::true_type{}, st + 1);
+    }
+#pragma unroll 1
+    for (; st < stages; st += 2) {
+        stage(std::integral_constant<int, 0>{}, std::false_type{}, st);
+        if (st + 1 < stages) stage(std::integral_constant<int, 1>{}, std::false_type{}, st + 1);
+    }
+
+    if constexpr (KS > 1) {  // the first team adds the others' sums, in their order
+        __syncthreads();
+        f32x4_t* const part = (f32x4_t*)lds;
+#pragma unroll
+        for (int k = 1; k < KS; ++k) {
+            const int at = ((k - 1) * T::TEAM + wave) * TW * TX * 256;
+#pragma unroll
+            for (int i = 0; i < TW; ++i)
+#pragma unroll
+                for (int j = 0; j < TX; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (team == k) part[at + ((i * TX + j) * 4 + q) * 64 + lane] = f32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
+        __syncthreads();
+        if (team != 0) return;
+#pragma unroll
+        for (int k = 1; k < KS; ++k) {
+            const int at = ((k - 1) * T::TEAM + wave) * TW * TX * 256;
+#pragma unroll
+            for (int i = 0; i < TW; ++i)
+#pragma unroll
+                for (int j = 0; j < TX; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const f32x4_t o = part[at + ((i * TX + j) * 4 + q) * 64 + lane];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += o[e];
+                    }
+        }
+    }
+
+    // epilogue: a wave turns 32 rows of its columns at a time through LDS, so that rows are stored in runs
+    if constexpr (KS == 1) __syncthreads();
+    constexpr int COLS = 32 * TW, PITCH = COLS + 4, OUT = GATED ? COLS / 2 : COLS, LPR = OUT / 8;  // LPR lanes store a row, 8 columns each
+    float* et = (float*)(lds + T::JOIN) + wave * 32 * PITCH;
+    const int c8 = (lane % LPR) * 8, n = n0 + wn * OUT + c8;
+#pragma unroll
+    for (int j = 0; j < TX; ++j) {
+#pragma unroll
+        for (int i = 0; i < TW; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *(f32x4_t*)(et + r * PITCH + i * 32 + q * 8 + h * 4) = f32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 2
+        for (int row = lane / LPR; row < 32; row += 64 / LPR) {
+            const int m = m0 + wm * 32 * TX + j * 32 + row;
+            if (m >= a.M || n >= a.N) continue;
+            float v[8], v2[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = et[row * PITCH + c8 + e];
+                v2[e] = GATED ? et[row * PITCH + OUT + c8 + e] : 0.f;
+            }
+            mx_store8(a, m, n, v, v2);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+// more LDS per workgroup than the 64 KB that need no leave; the leave is the device's own copy of the kernel's
+template <auto Kernel>
+hipError_t allow_lds(int bytes) {
+    static std::atomic<uint64_t> done[4];
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess || (dev < 256 && (done[dev >> 6].load(std::memory_order_relaxed) >> (dev & 63) & 1))) return e;
+    e = hipFuncSetAttribute((const void*)Kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess && dev < 256) done[dev >> 6].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
+    return e;
+}
+
+template <bool X4, int KS, int WN, int WM, int TW, int TX, bool GATED>
+hipError_t launch_tiles(hipStream_t s, MxArgs a) {
+    typedef Tile<X4, KS, WN, WM, TW, TX> T;
+    constexpr int NOUT = GATED ? T::BN / 2 : T::BN;
+    const uint32_t tiles_m = (uint32_t)((a.M + T::BM - 1) / T::BM);
+    a.tiles_n = (uint32_t)((a.N + NOUT - 1) / NOUT);
+    constexpr auto kernel = mx_tile_kernel<X4, KS, WN, WM, TW, TX, GATED>;
+    const hipError_t e = allow_lds<kernel>(T::LDS);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3(tiles_m * a.tiles_n), dim3(T::THREADS), T::LDS, s, a);
+    return hipGetLastError();
+}
+
+template <bool X4, bool GATED, int MT, int NT>
+hipError_t launch_rows(hipStream_t s, MxArgs a) {
+    constexpr int LDS = MX_WAVES * (GATED ? 2 : 1) * MT * NT * 1024;
+    constexpr auto kernel = mx_rows_kernel<X4, GATED, MT, NT>;
+    const hipError_t e = LDS > 64 * 1024 ? allow_lds<kernel>(LDS) : hipSuccess;
+    if (e != hipSuccess) return e;
+    a.tiles_n = (uint32_t)((a.N + 16 * NT - 1) / (16 * NT));
+    const int64_t rows_per_launch = std::max<int64_t>(1, 0x7FFFFFFF / (int64_t)a.tiles_n / (16 * MT)) * (16 * MT);  // a grid is below 2^31 workgroups
     const int M = a.M;
-    const int64_t x_row = x4 ? (int64_t)a.nb * 16 : a.ldx * 2, y_row = (int64_t)a.N * (a.out_f32 ? 4 : 2);
+    const int64_t x_row = X4 ? (int64_t)a.nb * 16 : a.ldx * 2, y_row = (int64_t)a.N * (a.out_f32 ? 4 : 2);
     for (int64_t m0 = 0; m0 < M; m0 += rows_per_launch) {
         MxArgs b = a;
         b.M = (int)std::min<int64_t>(M - m0, rows_per_launch);
         b.x = (const char*)a.x + m0 * x_row;
-        if (x4) b.xs = a.xs + m0 * a.nb;
+        if (X4) b.xs = a.xs + m0 * a.nb;
         if (a.res) b.res = (const char*)a.res + m0 * y_row;
         b.out = (char*)a.out + m0 * y_row;
-        const dim3 grid(a.tiles_n * (uint32_t)((b.M + 15) / 16)), block(64 * MX_WAVES);
-        if (x4 && a.w2) hipLaunchKernelGGL((mx_rows_kernel<true, true>), grid, block, 0, s, b);
-        else if (x4) hipLaunchKernelGGL((mx_rows_kernel<true, false>), grid, block, 0, s, b);
-        else if (a.w2) hipLaunchKernelGGL((mx_rows_kernel<false, true>), grid, block, 0, s, b);
-        else hipLaunchKernelGGL((mx_rows_kernel<false, false>), grid, block, 0, s, b);
+        hipLaunchKernelGGL(kernel, dim3(a.tiles_n * (uint32_t)((b.M + 16 * MT - 1) / (16 * MT))), dim3(64 * MX_WAVES), LDS, s, b);
     }
     return hipGetLastError();
+}
+
+// Estimated microseconds of the two kernels, in the coefficients that a fit to 180 measured products gives (1 .. 2048 rows, 100 .. 16384 columns, K from
+// 300 to 8192; the choice by them costs 2 - 3 % over the best one on average).  A workgroup of the first kernel reads its rows of x and of the
+// weights; what counts is how much a CU reads.  One of the second advances by stages, a little slower when all CUs work.
+template <bool X4>
+double rows_us(const MxArgs& a, int mt, int nt) {
+    const double mats = a.w2 ? 2 : 1, wgs = (double)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt));
+    const double kb = 1e-3 * a.nb * (std::min(a.M, 16 * mt) * (X4 ? 17 : 64) + 16 * nt * mats * 17);
+    return (X4 ? 2.5 : 2.9) + (X4 ? 0.155 : 0.26) * mt * nt * mats + (X4 ? 0.046 : 0.034) * kb * std::max(1.0, wgs / 256);
+}
+template <bool X4>
+double tiles_us(const MxArgs& a, int edge) {
+    const double tiles = (double)((a.M + edge - 1) / edge) * (((a.w2 ? 2.0 : 1.0) * a.N + edge - 1) / edge), rounds = std::ceil(tiles / 256);
+    const double full = std::min(1.0, tiles / 256), blocks = a.nb;
+    if (edge == 128) return X4 ? 2.1 + rounds * (3.0 + blocks * (0.056 + 0.049 * full)) : 2.3 + rounds * (3.8 + blocks * (0.168 + 0.1 * full));
+    return X4 ? 7.0 + rounds * blocks * (0.176 + 0.144 * full) : 10.4 + rounds * (blocks * (0.54 + 0.3 * full) - 0.9);
+}
+
+template <bool X4, bool GATED>
+hipError_t choose(hipStream_t s, const MxArgs& a) {
+    const double r11 = rows_us<X4>(a, 1, 1), r12 = rows_us<X4>(a, 1, 2), r14 = rows_us<X4>(a, 1, 4), r22 = rows_us<X4>(a, 2, 2), r24 = rows_us<X4>(a, 2, 4);
+    const double rows = std::min({r11, r12, r14, r22, r24});
+    const int64_t x_row = X4 ? (int64_t)a.nb * 16 : a.ldx * 2;
+    // the second kernel counts bytes within a workgroup's rows, and workgroups, in 32 bits
+    if (x_row <= 1 << 23 && a.nb <= 1 << 19 && (double)a.M * a.N < 1e13) {
+        const double t128 = tiles_us<X4>(a, 128), t256 = tiles_us<X4>(a, 256);
+        if (t256 < t128 && t256 < rows) return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
+        if (t128 < rows) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
+    }
+    if (r11 == rows) return launch_rows<X4, GATED, 1, 1>(s, a);
+    if (r12 == rows) return launch_rows<X4, GATED, 1, 2>(s, a);
+    if (r14 == rows) return launch_rows<X4, GATED, 1, 4>(s, a);
+    if (r22 == rows) return launch_rows<X4, GATED, 2, 2>(s, a);
+    return launch_rows<X4, GATED, 2, 4>(s, a);
+}
+
+hipError_t launch_products(hipStream_t s, MxArgs a, bool x4) {
+    a.x_direct = x4 || (op_aligned(a.x, 4) && a.ldx % 2 == 0);
+    a.s_direct = a.nb % 4 == 0 && op_aligned(a.ws, 4) && op_aligned(a.ws2, 4) && op_aligned(a.xs, 4);
+    return x4 ? (a.w2 ? choose<true, true>(s, a) : choose<true, false>(s, a)) : (a.w2 ? choose<false, true>(s, a) : choose<false, false>(s, a));
 }
 
 // the checks that both products share; null: fine
 const char* product_fault(int32_t M, int32_t N, int32_t K, const void* codes, const void* scales, const void* codes2, const void* scales2, const void* bias,
                           const void* bias2, const void* residual, int32_t out_dtype, const void* out) {
     if (M < 0 || N < 0 || K < 1) return "M and N must not be negative, K must be positive";
-    if (K > 0x7FFFFFFF - 4096) return "K is too large";
+    if (std::max({M, N, K}) > 0x7FFFFFFF - 4096) return "M, N or K is too large";
     if (out_dtype != MV_BF16 && out_dtype != MV_F32) return "out_dtype must be MV_BF16 or MV_F32";
     if (M == 0 || N == 0) return nullptr;
     if (!codes || !scales || !out) return "null argument";
@@ -308,7 +839,7 @@ int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void
     OpDevice dev((hipStream_t)stream, out);
     MX_TRY(dev.status());
     MxArgs a{x, nullptr, (const unsigned char*)codes, (const unsigned char*)scales, (const unsigned char*)codes2, (const unsigned char*)scales2,
-             (const bf16_t*)bias, (const bf16_t*)bias2, residual, out, ldx, M, N, K, (K + 31) / 32, out_dtype == MV_F32, 0};
+             (const bf16_t*)bias, (const bf16_t*)bias2, residual, out, ldx, M, N, K, (K + 31) / 32, out_dtype == MV_F32, 0, 0, 0};
     MX_TRY(launch_products((hipStream_t)stream, a, false));
     return MV_OK;
 }
@@ -322,7 +853,7 @@ int mv_op_gemm_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* 
     OpDevice dev((hipStream_t)stream, out);
     MX_TRY(dev.status());
     MxArgs a{x_codes, (const unsigned char*)x_scales, (const unsigned char*)codes, (const unsigned char*)scales, (const unsigned char*)codes2,
-             (const unsigned char*)scales2, (const bf16_t*)bias, (const bf16_t*)bias2, residual, out, 0, M, N, K, (K + 31) / 32, out_dtype == MV_F32, 0};
+             (const unsigned char*)scales2, (const bf16_t*)bias, (const bf16_t*)bias2, residual, out, 0, M, N, K, (K + 31) / 32, out_dtype == MV_F32, 0, 0, 0};
     MX_TRY(launch_products((hipStream_t)stream, a, true));
     return MV_OK;
 }

@@ -47,6 +47,7 @@ def gemm(m=4, n=8, k=64, x=A, xs=A, codes=A, scales=A, codes2=None, scales2=None
 
 @pytest.mark.parametrize("fn", [linear, gemm])
 @pytest.mark.parametrize("kw,text", [(dict(m=-1), "negative"), (dict(n=-1), "negative"), (dict(k=0), "positive"), (dict(k=-5), "positive"),
+                                     (dict(m=2 ** 31 - 1), "too large"), (dict(n=2 ** 31 - 1), "too large"),
                                      (dict(out_dtype=2), "out_dtype"), (dict(codes=None), "null"), (dict(scales=None), "null"), (dict(out=None), "null"),
                                      (dict(x=None), "x"), (dict(codes2=A), "together"), (dict(scales2=A), "together"), (dict(bias2=A), "bias2"),
                                      (dict(codes=A + 4), "16 bytes"), (dict(codes2=A + 4, scales2=A), "16 bytes"), (dict(out=A + 1), "element"),
