@@ -39,7 +39,7 @@ struct ControlArgs {
     int32_t* allowed;
     int64_t ld, ld_out;
     int32_t vocab;
-    uint32_t chunks;  // per row
+    uint32_t chunks, groups;  // chunks of a row, and its workgroups: one more where the mask's bits are counted
 };
 
 // 4 consecutive logits of a row from token v on, zero past the vocabulary
@@ -65,55 +65,85 @@ __device__ __forceinline__ f32x4_t lc_load(const void* base, int64_t at, int lef
     return r;
 }
 
+#define LC_AHEAD 4  // history ids per thread that are asked for at once
+
 template <bool IN32, bool OUT32>
 __global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const ControlArgs a) {
     __shared__ __attribute__((aligned(16))) uint32_t count[LC_CHUNK];  // bit 31: in the prompt; below: occurrences behind it
     __shared__ __attribute__((aligned(16))) uint32_t entry[LC_CHUNK];  // 1 + the bias entry that holds, 0: none
-    __shared__ int n_allowed;
     const mv_logit_controls& c = a.c;
     const int tid = threadIdx.x;
-    const uint32_t row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks;
+    const uint32_t row = blockIdx.x / a.groups, chunk = blockIdx.x - row * a.groups;
+    const int index = c.masks == nullptr ? -1 : c.mask_index ? c.mask_index[row] : (int)row;
+    const uint32_t* mask = index >= 0 && index < c.n_masks ? c.masks + (int64_t)index * c.ld_mask : nullptr;
+
+    if (chunk == a.chunks) {  // behind the chunks of a row: a workgroup that counts the bits of its mask
+        int n = 0;
+        if (mask) {
+#pragma unroll 4
+            for (int w = tid; w < (a.vocab + 31) / 32; w += LC_THREADS) {
+                const int left = a.vocab - w * 32;
+                n += __popc(left >= 32 ? mask[w] : mask[w] & ((1u << left) - 1u));
+            }
+        } else if (tid == 0) n = a.vocab;
+        if (tid == 0) count[0] = 0;
+        __syncthreads();
+        if (n) atomicAdd(&count[0], (uint32_t)n);
+        __syncthreads();
+        if (tid == 0) a.allowed[row] = (int32_t)count[0];
+        return;
+    }
+
+    // Everything that depends on nothing else is asked for first: logits, mask words, the first history and bias ids (a history's room is readable
+    // whatever its length), so that the two rounds over LDS wait for memory once.
     const int v0 = (int)(chunk * LC_CHUNK);
     const bool counted = c.history != nullptr, biased = c.bias_ids != nullptr;
-
-    // the logits are on their way while the words are gathered
+    const int len = !counted ? 0 : c.history_len ? min(max(c.history_len[row], 0), c.history_cap) : c.history_cap;
+    const int prompt = counted && c.prompt_len ? c.prompt_len[row] : 0;
+    const int32_t* h = c.history + (int64_t)row * c.ld_history;
+    const int32_t* ids = c.bias_ids + (int64_t)row * c.ld_bias;
     f32x4_t x[LC_GROUPS], u[LC_GROUPS];
+    uint32_t word[LC_GROUPS];
 #pragma unroll
     for (int j = 0; j < LC_GROUPS; ++j) {
         const int v = v0 + (j * LC_THREADS + tid) * 4, left = a.vocab - v;
         x[j] = left > 0 ? lc_load<IN32>(a.logits, (int64_t)row * a.ld + v, left) : f32x4_t{0, 0, 0, 0};
         u[j] = left > 0 && a.uncond ? lc_load<IN32>(a.uncond, (int64_t)row * a.ld + v, left) : f32x4_t{0, 0, 0, 0};
+        word[j] = left > 0 && mask ? mask[v >> 5] : 0xFFFFFFFFu;
     }
-    const uint32_t* mask = nullptr;
-    if (c.masks) {
-        const int index = c.mask_index ? c.mask_index[row] : (int)row;
-        if (index >= 0 && index < c.n_masks) mask = c.masks + (int64_t)index * c.ld_mask;
-    }
+    int seen[LC_AHEAD], extra = -1;
+#pragma unroll
+    for (int k = 0; k < LC_AHEAD; ++k) seen[k] = counted && tid + k * LC_THREADS < c.history_cap ? h[tid + k * LC_THREADS] : -1;
+    if (biased && tid < c.n_bias) extra = ids[tid];
 
     if (counted || biased) {
 #pragma unroll
         for (int j = 0; j < LC_GROUPS; ++j) {
-            *(u32x4*)&count[(j * LC_THREADS + tid) * 4] = u32x4{0, 0, 0, 0};
+            if (counted) *(u32x4*)&count[(j * LC_THREADS + tid) * 4] = u32x4{0, 0, 0, 0};
             if (biased) *(u32x4*)&entry[(j * LC_THREADS + tid) * 4] = u32x4{0, 0, 0, 0};
         }
         __syncthreads();
+        const uint32_t width = (uint32_t)min(LC_CHUNK, a.vocab - v0);
+        const auto note = [&](int id, int i) {
+            const uint32_t k = (uint32_t)id - (uint32_t)v0;
+            if (i >= len || k >= width) return;
+            if (i < prompt) atomicOr(&count[k], 0x80000000u);
+            else atomicAdd(&count[k], 1u);
+        };
         if (counted) {
-            const int len = c.history_len ? min(max(c.history_len[row], 0), c.history_cap) : c.history_cap;
-            const int prompt = c.prompt_len ? c.prompt_len[row] : 0;
-            const int32_t* h = c.history + (int64_t)row * c.ld_history;
-            for (int i = tid; i < len; i += LC_THREADS) {
-                const int id = h[i];
-                if (id >= v0 && id < a.vocab && id - v0 < LC_CHUNK) {
-                    if (i < prompt) atomicOr(&count[id - v0], 0x80000000u);
-                    else atomicAdd(&count[id - v0], 1u);
-                }
+#pragma unroll
+            for (int k = 0; k < LC_AHEAD; ++k) note(seen[k], tid + k * LC_THREADS);
+            for (int i = tid + LC_AHEAD * LC_THREADS; i < len; i += LC_AHEAD * LC_THREADS) {
+#pragma unroll
+                for (int k = 0; k < LC_AHEAD; ++k) seen[k] = i + k * LC_THREADS < len ? h[i + k * LC_THREADS] : -1;
+#pragma unroll
+                for (int k = 0; k < LC_AHEAD; ++k) note(seen[k], i + k * LC_THREADS);
             }
         }
         if (biased) {
-            const int32_t* ids = c.bias_ids + (int64_t)row * c.ld_bias;
             for (int i = tid; i < c.n_bias; i += LC_THREADS) {
-                const int id = ids[i];
-                if (id >= v0 && id < a.vocab && id - v0 < LC_CHUNK) atomicMax(&entry[id - v0], (uint32_t)i + 1u);
+                const uint32_t k = (uint32_t)(i == tid ? extra : ids[i]) - (uint32_t)v0;
+                if (k < width) atomicMax(&entry[k], (uint32_t)i + 1u);
             }
         }
         __syncthreads();
@@ -146,12 +176,10 @@ __global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const Contro
             for (int i = 0; i < 4; ++i)
                 if (e4[i]) x[j][i] += c.bias[(int64_t)row * c.ld_bias + e4[i] - 1];
         }
-        if (mask) {
-            const uint32_t bits = mask[v >> 5] >> (v & 31);
+        const uint32_t bits = word[j] >> (v & 31);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (!((bits >> i) & 1)) x[j][i] = -INFINITY;
-        }
+        for (int i = 0; i < 4; ++i)
+            if (!((bits >> i) & 1)) x[j][i] = -INFINITY;
         const int64_t at = (int64_t)row * a.ld_out + v;
         if (OUT32) {
             float* o = (float*)a.out + at;
@@ -165,21 +193,6 @@ __global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const Contro
                 for (int i = 0; i < left; ++i) o[i] = f2bf(x[j][i]);
         }
     }
-
-    if (a.allowed != nullptr && chunk == 0) {  // the first chunk's workgroup counts the bits of the whole mask
-        int n = 0;
-        if (mask) {
-            for (int w = tid; w < (a.vocab + 31) / 32; w += LC_THREADS) {
-                const int left = a.vocab - w * 32;
-                n += __popc(left >= 32 ? mask[w] : mask[w] & ((1u << left) - 1u));
-            }
-        } else if (tid == 0) n = a.vocab;
-        if (tid == 0) n_allowed = 0;
-        __syncthreads();
-        if (n) atomicAdd(&n_allowed, n);
-        __syncthreads();
-        if (tid == 0) a.allowed[row] = n_allowed;
-    }
 }
 
 }  // namespace
@@ -191,7 +204,7 @@ extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, i
         return mv_fail(MV_ERR_INVALID, "logit_controls: dtype %d -> %d (MV_BF16 or MV_F32)", dtype, out_dtype);
     if (ld < vocab || ld_out < vocab) return mv_fail(MV_ERR_INVALID, "logit_controls: a row stride (%lld, %lld) is below the vocabulary %d", (long long)ld, (long long)ld_out, vocab);
     if (!controls) return mv_fail(MV_ERR_INVALID, "logit_controls: null argument");
-    ControlArgs a{*controls, logits, uncond, out, allowed, ld, ld_out, vocab, 0};
+    ControlArgs a{*controls, logits, uncond, out, allowed, ld, ld_out, vocab, 0, 0};
     mv_logit_controls& c = a.c;
     if (uncond && !c.guidance) return mv_fail(MV_ERR_INVALID, "logit_controls: uncond without guidance");
     if (c.history_cap < 0 || c.n_bias < 0 || c.n_masks < 0) return mv_fail(MV_ERR_INVALID, "logit_controls: a negative count");
@@ -209,10 +222,11 @@ extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, i
     if (c.history_cap == 0 || (!c.repetition && !c.presence && !c.frequency)) c.history = nullptr;
     if (c.n_bias == 0) c.bias_ids = nullptr;
     a.chunks = (uint32_t)((vocab + (int64_t)LC_CHUNK - 1) / LC_CHUNK);
-    if ((int64_t)a.chunks * rows > 0x7FFFFFFF) return mv_fail(MV_ERR_INVALID, "logit_controls: rows=%d vocab=%d is too large", rows, vocab);
+    a.groups = a.chunks + (allowed ? 1 : 0);
+    if ((int64_t)a.groups * rows > 0x7FFFFFFF) return mv_fail(MV_ERR_INVALID, "logit_controls: rows=%d vocab=%d is too large", rows, vocab);
     OpDevice dev((hipStream_t)stream, out);
     LC_TRY(dev.status());
-    const dim3 grid(a.chunks * (uint32_t)rows), block(LC_THREADS);
+    const dim3 grid(a.groups * (uint32_t)rows), block(LC_THREADS);
     if (dtype == MV_F32 && out_dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<true, true>), grid, block, 0, (hipStream_t)stream, a);
     else if (dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<true, false>), grid, block, 0, (hipStream_t)stream, a);
     else if (out_dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<false, true>), grid, block, 0, (hipStream_t)stream, a);
