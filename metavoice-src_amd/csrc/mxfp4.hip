@@ -200,6 +200,7 @@ __device__ __forceinline__ bf16x8_t mx_widen(uint32_t q, float scale) {
     return __builtin_bit_cast(bf16x8_t, r);
 }
 
+#define MX_INLINE __attribute__((always_inline))
 #define MX_WAVES 8
 
 // Few rows: one workgroup computes 16 MT rows of x against 16 NT weight rows; its waves take the 128-column steps of K in turn, each straight from memory
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
     const int wm = wave % WM, wn = wave / WM;
     constexpr int NOUT = GATED ? T::BN / 2 : T::BN;  // output columns of a workgroup
 
-    // workgroups go round the 8 XCDs: each XCD takes a contiguous range of tiles, ordered in bands of 8 row tiles so that the tiles in flight on it
+    // workgroups go round the 8 XCDs: each XCD takes a contiguous range of tiles, ordered in bands of 4 row tiles so that the 32 tiles in flight on it
     // share rows of x and of the weights in its L2
     uint32_t id = blockIdx.x;
     {
@@ -371,11 +372,11 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
         id = xcd * q + min(xcd, rem) + k;
     }
     const uint32_t tiles_m = (uint32_t)((a.M + T::BM - 1) / T::BM);
-    const uint32_t band = id / (8 * a.tiles_n), in_band = id - band * 8 * a.tiles_n, rows_in = min(8u, tiles_m - band * 8);
-    const int m0 = (int)(band * 8 + in_band % rows_in) * T::BM, n0 = (int)(in_band / rows_in) * NOUT;
+    const uint32_t band = id / (4 * a.tiles_n), in_band = id - band * 4 * a.tiles_n, rows_in = min(4u, tiles_m - band * 4);
+    const int m0 = (int)(band * 4 + in_band % rows_in) * T::BM, n0 = (int)(in_band / rows_in) * NOUT;
 
     // row of the weights' LDS image -> matrix and weight row (gated: a wave's first half of columns from w, the second half the same columns of w2)
-    auto w_row = [&](int row, int& second) {
+    auto w_row = [&](int row, int& second) MX_INLINE {
         if (!GATED) { second = 0; return min(n0 + row, a.N - 1); }
         second = (row / (16 * TW)) & 1;
         return min(n0 + (row / (32 * TW)) * (16 * TW) + row % (16 * TW), a.N - 1);
@@ -401,34 +402,27 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
         wbase[i] = (second ? a.w2 : a.w) + (int64_t)n0 * code_row;
     }
     const int stages = (a.nb + KS * T::BLOCKS - 1) / (KS * T::BLOCKS);
-    const int direct = a.x_direct ? (X4 ? a.nb / (KS * 8) : a.K / (KS * 64)) : 0;  // the stages that are whole and aligned
+    const int whole = X4 ? a.nb / (KS * 8) : a.K / (KS * 64), direct = a.x_direct ? whole : 0;  // the stages that are not short; and aligned
 
     const int share = team * T::SHARE;
-    auto transfer = [&](int st, int buf) {
+    auto transfer_x = [&](int st, int buf) MX_INLINE {
         const int v = st * KS + team;
 #pragma unroll
         for (int i = 0; i < T::XI; ++i)
             __builtin_amdgcn_global_load_lds((glb_ptr_t)(xbase + (int64_t)v * T::XROW + gx[i]), (lds_ptr_t)(lds + buf + share + (wave * T::XI + i) * 1024), 16, 0, 0);
+    };
+    auto transfer_w = [&](int st, int buf) MX_INLINE {
+        const int v = st * KS + team;
 #pragma unroll
         for (int i = 0; i < T::WI; ++i)
             __builtin_amdgcn_global_load_lds((glb_ptr_t)(wbase[i] + (int64_t)v * T::WROW + gw[i]), (lds_ptr_t)(lds + buf + share + T::X + (wave * T::WI + i) * 1024), 16, 0, 0);
     };
-    // the short stage at the end of a row, and rows of x that are not aligned: through registers, zeros past K
-    auto carry = [&](int st, int buf) {
-        const int v = st * KS + team, t = tid % (64 * T::TEAM);
+    // What transfers cannot bring comes through registers, zeros past K: the short stage at the end of a row, and rows of bf16 that are not aligned to 4
+    // bytes.  The latter are asked for at one stage and put into LDS at the next (the larger tile has no registers for that and does not take them).
+    auto carry_w = [&](int st, int buf) MX_INLINE {
+        const int v = st * KS + team;
 #pragma unroll 1
-        for (int i = t; i < T::X / 16; i += 64 * T::TEAM) {
-            const int row = i / XCH, c = mx_slot<T::XROW>(row, i % XCH), m = min(m0 + row, a.M - 1);
-            u32x4 q = {0u, 0u, 0u, 0u};
-            if (X4) {
-                if (v * T::BLOCKS + c < a.nb) q = *(const u32x4*)((const unsigned char*)a.x + m * x_row + (int64_t)(v * T::BLOCKS + c) * 16);
-            } else {
-                q = mx_load_x8((const bf16_t*)a.x + m * a.ldx, v * 64 + c * 8, a.K);
-            }
-            *(u32x4*)(lds + buf + share + i * 16) = q;
-        }
-#pragma unroll 1
-        for (int i = t; i < T::W / 16; i += 64 * T::TEAM) {
+        for (int i = tid % (64 * T::TEAM); i < T::W / 16; i += 64 * T::TEAM) {
             const int row = i / WCH, c = mx_slot<T::WROW>(row, i % WCH);
             int second;
             const int n = w_row(row, second);
@@ -437,9 +431,31 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
             *(u32x4*)(lds + buf + share + T::X + i * 16) = q;
         }
     };
+    auto x_piece = [&](int st, int at) MX_INLINE {  // 16 bytes of a stage's x in the order of its LDS image
+        const int v = st * KS + team, row = at / XCH, c = mx_slot<T::XROW>(row, at % XCH), m = min(m0 + row, a.M - 1);
+        if (X4) return v * T::BLOCKS + c < a.nb ? *(const u32x4*)((const unsigned char*)a.x + m * x_row + (int64_t)(v * T::BLOCKS + c) * 16) : u32x4{0u, 0u, 0u, 0u};
+        const bf16_t* p = (const bf16_t*)a.x + m * a.ldx;
+        return (v + 1) * 64 <= a.K ? (u32x4) * (const u32x4_any*)(p + v * 64 + c * 8) : mx_load_x8(p, v * 64 + c * 8, a.K);
+    };
+    auto carry_x = [&](int st, int buf) MX_INLINE {
+#pragma unroll 1
+        for (int i = tid % (64 * T::TEAM); i < T::X / 16; i += 64 * T::TEAM) *(u32x4*)(lds + buf + share + i * 16) = x_piece(st, i);
+    };
+    constexpr bool LATER = KS > 1;
+    constexpr int XC = LATER ? T::X / 1024 / T::TEAM : 0;  // 16-byte pieces of x per thread and stage
+    u32x4 xreg[XC + 1];
+    auto x_in = [&](int st) MX_INLINE {
+#pragma unroll
+        for (int i = 0; i < XC; ++i) xreg[i] = x_piece(st, tid % (64 * T::TEAM) + i * 64 * T::TEAM);
+    };
+    auto x_out = [&](int buf) MX_INLINE {
+#pragma unroll
+        for (int i = 0; i < XC; ++i) *(u32x4*)(lds + buf + share + (tid % (64 * T::TEAM) + i * 64 * T::TEAM) * 16) = xreg[i];
+    };
+
     // scales of a group: 16 bytes of row t (with 4-bit x the rows of x come first) by transfer t / 64, wave after wave
     constexpr int SBASE = NBUF * T::STAGE, SN = T::SROWS / 64, SI = (SN + T::WAVES - 1) / T::WAVES;
-    auto scale_row = [&](int row) {
+    auto scale_row = [&](int row) MX_INLINE {
         if (X4 && row < T::BM) return a.xs + (int64_t)min(m0 + row, a.M - 1) * a.nb;
         int second;
         const int n = w_row(X4 ? row - T::BM : row, second);
@@ -449,8 +465,8 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
 #pragma unroll
     for (int i = 0; i < SI; ++i) gs[i] = scale_row(min(wave_of_all + i * T::WAVES, SN - 1) * 64 + lane);
     const int whole_groups = a.nb / 16;
-    auto scale_at = [&](int group) { return SBASE + (group >= whole_groups ? T::RING : group % T::RING) * T::S; };
-    auto scales = [&](int group) {  // a whole, aligned group
+    auto scale_at = [&](int group) MX_INLINE { return SBASE + (group >= whole_groups ? T::RING : group % T::RING) * T::S; };
+    auto scales = [&](int group) MX_INLINE {  // a whole, aligned group
         const int to = scale_at(group);
 #pragma unroll
         for (int i = 0; i < SI; ++i)
@@ -460,11 +476,11 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
     // whole groups of rows of scales that are not aligned to 4 bytes: through registers, asked for at one stage and put into LDS at the next
     u32x4 sreg = {0u, 0u, 0u, 0u};
     static_assert(T::SROWS <= T::THREADS, "a row of scales per thread");
-    auto scales_in = [&](int group) { sreg = *(const u32x4_byte*)(scale_row(min(tid, T::SROWS - 1)) + group * 16); };
-    auto scales_out = [&](int group) {
+    auto scales_in = [&](int group) MX_INLINE { sreg = *(const u32x4_byte*)(scale_row(min(tid, T::SROWS - 1)) + group * 16); };
+    auto scales_out = [&](int group) MX_INLINE {
         if (tid < T::SROWS) *(u32x4*)(lds + scale_at(group) + tid * 16) = sreg;
     };
-    auto carry_scales = [&](int group) {  // at the start: a short group at the end of a row
+    auto carry_scales = [&](int group) MX_INLINE {  // at the start: a short group at the end of a row
         const int b = group * 16, to = scale_at(group);
 #pragma unroll 1
         for (int i = tid; i < T::SROWS * 4; i += T::THREADS) {
@@ -492,15 +508,15 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
         xat[t] = share + (wm * 32 * TX + r) * T::XROW + mx_slot<T::XROW>(r, T::STEPS * h + t) * 16;
         if (X4 || t == 0) wat[X4 ? t : 0] = share + T::X + (wn * 32 * TW + r) * T::WROW + mx_slot<T::WROW>(r, X4 ? T::STEPS * h + t : h) * 16;
     }
-    auto read_x = [&](int buf, int t, u32x4 (&f)[TX]) {
+    auto read_x = [&](int buf, int t, u32x4 (&f)[TX]) MX_INLINE {
 #pragma unroll
         for (int j = 0; j < TX; ++j) f[j] = *(const u32x4*)(lds + buf + xat[t] + j * 32 * T::XROW);
     };
-    auto read_w = [&](int buf, int t, u32x4 (&f)[TW]) {
+    auto read_w = [&](int buf, int t, u32x4 (&f)[TW]) MX_INLINE {
 #pragma unroll
         for (int i = 0; i < TW; ++i) f[i] = *(const u32x4*)(lds + buf + wat[X4 ? t : 0] + i * 32 * T::WROW);
     };
-    auto read_s = [&](int st, uint32_t (&fsx)[TX], uint32_t (&fsw)[TW]) {
+    auto read_s = [&](int st, uint32_t (&fsx)[TX], uint32_t (&fsw)[TW]) MX_INLINE {
         const unsigned char* buf = lds + scale_at(st / T::GROUP) + (st % T::GROUP * KS + team) * T::BLOCKS + (X4 ? h * 4 : h) + r * 16;
         if (X4) {
 #pragma unroll
@@ -515,7 +531,7 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
     // The products of a step.  They stay where they stand: left alone, the compiler carries them past the branches and reads of later steps, with all
     // the registers that takes.
     // The reads of the next step (`reads`) come behind the first products: the compiler waits for all reads on their way where it waits for one.
-    auto multiply = [&](auto step, const u32x4 (&x)[TX], const u32x4 (&w)[TW], const uint32_t (&csx)[TX], const uint32_t (&csw)[TW], auto reads) {
+    auto multiply = [&](auto step, const u32x4 (&x)[TX], const u32x4 (&w)[TW], const uint32_t (&csx)[TX], const uint32_t (&csw)[TW], auto reads) MX_INLINE {
         constexpr int t = decltype(step)::value;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -552,8 +568,14 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
         if (a.s_direct && i < whole_groups) scales(i);
 #pragma unroll
     for (int i = 0; i < NBUF; ++i) {
-        if (i < direct) transfer(i, i * T::STAGE);
-        else if (i < stages) carry(i, i * T::STAGE);
+        if (i >= stages) break;
+        if (i < whole) transfer_w(i, i * T::STAGE);
+        else carry_w(i, i * T::STAGE);
+        if (i < direct) {
+            transfer_x(i, i * T::STAGE);
+        } else {
+            carry_x(i, i * T::STAGE);
+        }
     }
     if (a.nb % 16) carry_scales(whole_groups);
     if (!a.s_direct)
@@ -569,18 +591,32 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
     read_x(0, 0, fx[0]);
 
     int cur = 0;  // byte offset of the stage's buffer
-    const auto wait_and_ask = [&](auto kind, int st) {
+    const auto wait_and_ask = [&](auto kind, int st) MX_INLINE {
         constexpr bool DIRECT = decltype(kind)::value;
-        if (!DIRECT && !a.s_direct && (st - 1) % T::GROUP == 0 && st > 0 && (st - 1) / T::GROUP + T::AHEAD < whole_groups) scales_out((st - 1) / T::GROUP + T::AHEAD);
+        if (!DIRECT && st > 0) {  // what stage st - 1 asked for: its buffer, and a place for scales
+            if (LATER && st - 1 + NBUF >= direct && st - 1 + NBUF < stages) x_out(cur == 0 ? (NBUF - 1) * T::STAGE : cur - T::STAGE);
+            if (!a.s_direct && (st - 1) % T::GROUP == 0 && (st - 1) / T::GROUP + T::AHEAD < whole_groups) scales_out((st - 1) / T::GROUP + T::AHEAD);
+        }
         // stage st + 1 must have arrived, NBUF - 2 later ones may be on their way (a request for scales among them only makes the wait longer)
         if (st + NBUF - 1 < direct) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NBUF - 2) * (T::XI + T::WI)) : "memory");
+        else if (!DIRECT && st + NBUF - 1 < whole) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NBUF - 2) * T::WI) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         // and every wave has read all of stage st: its buffer is free
-        if (st + NBUF < direct) transfer(st + NBUF, cur);
-        else if (!DIRECT && st + NBUF < stages) carry(st + NBUF, cur);
+        if (DIRECT) {
+            if (st + NBUF < direct) {
+                transfer_x(st + NBUF, cur);
+                transfer_w(st + NBUF, cur);
+            }
+        } else if (st + NBUF < stages) {
+            if (st + NBUF < direct) transfer_x(st + NBUF, cur);
+            else if (LATER) x_in(st + NBUF);
+            else carry_x(st + NBUF, cur);
+            if (st + NBUF < whole) transfer_w(st + NBUF, cur);
+            else carry_w(st + NBUF, cur);
+        }
         if (st % T::GROUP == 0 && st / T::GROUP + T::AHEAD < whole_groups) {
             if (DIRECT || a.s_direct) scales(st / T::GROUP + T::AHEAD);
             else scales_in(st / T::GROUP + T::AHEAD);
@@ -588,7 +624,7 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
     };
     // A stage, P its parity.  DIRECT: all that it asks for comes without registers.  (In one loop with the other kind, the compiler would let every read
     // of LDS wait for all that are on their way.)
-    auto stage = [&](auto parity, auto kind, int st) {
+    auto stage = [&](auto parity, auto kind, int st) MX_INLINE {
         constexpr int P = decltype(parity)::value;
         const int next = cur + T::STAGE == NBUF * T::STAGE ? 0 : cur + T::STAGE;
         multiply(std::integral_constant<int, 0>{}, fx[0], fw[X4 ? 0 : P], sx[P], sw[P], [&] {
@@ -759,7 +795,7 @@ hipError_t choose(hipStream_t s, const MxArgs& a) {
     // the second kernel counts bytes within a workgroup's rows, and workgroups, in 32 bits
     if (x_row <= 1 << 23 && a.nb <= 1 << 19 && (double)a.M * a.N < 1e13) {
         const double t128 = tiles_us<X4>(a, 128), t256 = tiles_us<X4>(a, 256);
-        if (t256 < t128 && t256 < rows) return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
+        if (a.x_direct && t256 < t128 && t256 < rows) return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
         if (t128 < rows) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
     }
     if (r11 == rows) return launch_rows<X4, GATED, 1, 1>(s, a);

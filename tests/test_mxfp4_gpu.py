@@ -104,6 +104,15 @@ def make(g, n, k, spread=1.0):
     return codes, scales
 
 
+def make_fast(g, n, k):
+    """Random codes and scales, zeros past K."""
+    nb = o_mx.blocks(k)
+    q = torch.randint(0, 256, (n, 16 * nb), generator=g).numpy().astype(np.uint8)
+    cols = np.arange(32 * nb).reshape(-1, 2)
+    q &= ((cols[:, 0] < k) * 15 + (cols[:, 1] < k) * 240).astype(np.uint8)
+    return q, torch.randint(118, 128, (n, nb), generator=g).numpy().astype(np.uint8)
+
+
 def dev(a):
     return torch.from_numpy(a).cuda()
 
@@ -138,7 +147,7 @@ SHAPES = [(1, 1, 1), (1, 16, 32), (2, 2562, 2048), (3, 17, 33), (5, 40, 96), (16
           (65, 260, 512), (100, 1000, 736), (128, 128, 256), (130, 257, 511), (200, 512, 1024), (257, 300, 2080), (512, 520, 288), (300, 1030, 31)]
 
 
-def case(kind, m, n, k, gated, bias, residual, dtype, pad=0):
+def case(kind, m, n, k, gated, bias, residual, dtype, pad=0, make=make):
     g = torch.Generator().manual_seed(m * 7 + n * 3 + k)
     if kind == "linear":
         x = torch.randn(m, k + pad, generator=g).bfloat16().cuda()[:, :k]
@@ -164,6 +173,47 @@ def test_product(kind, m, n, k):
                                          (True, True, True, torch.bfloat16)):
         args, want, size = case(kind, m, n, k, gated, bias, residual, dtype)
         within(product(kind, **args), want, size, k, dtype)
+
+
+# Products large enough for the row kernels of several tiles and for both tiled kernels: whole and short stages, rows of scales that are and are not
+# aligned (ceil(K / 32) a multiple of 4 or not), ragged last tiles, an odd number of stages.
+LARGE = [(25, 6000, 1500), (30, 9000, 600), (700, 900, 1088), (600, 1500, 1100), (1100, 1300, 640), (1537, 4100, 320), (2049, 4100, 200), (1300, 6200, 1000),
+         (1100, 8300, 225), (2300, 3900, 289), (513, 2500, 2049), (3000, 3100, 1024)]
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+def test_large_product(kind, m, n, k):
+    for gated, bias, residual, dtype in ((False, False, False, torch.bfloat16), (True, True, True, torch.float32)):
+        args, want, size = case(kind, m, n // 2 if gated else n, k, gated, bias, residual, dtype, make=make_fast)
+        within(product(kind, **args), want, size, k, dtype)
+
+
+@pytest.mark.parametrize("pad", [1, 2, 8])
+@pytest.mark.parametrize("m,n,k", [(700, 900, 1088), (1100, 1300, 640), (1300, 6200, 1000), (2300, 3900, 289)])
+def test_large_linear_of_strided_rows(m, n, k, pad):
+    args, want, size = case("linear", m, n, k, False, True, False, torch.bfloat16, pad, make=make_fast)
+    within(product("linear", **args), want, size, k, torch.bfloat16)
+
+
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+def test_large_products_repeat_and_leave_nan_in_its_row(kind):
+    """Both tiled kernels: the same bits on every run; a NaN block reaches its own weight row, and with 4-bit x its own x row, and nothing else."""
+    for m, n, k in ((1100, 1300, 640), (2100, 4000, 416)):
+        args, _, _ = case(kind, m, n, k, False, False, False, torch.float32, make=make_fast)
+        first = product(kind, **args)
+        for _ in range(3):
+            assert torch.equal(product(kind, **args), first)
+        args["w"][1][n - 3, 5] = 255
+        if kind == "gemm":
+            args["x"][1][m - 2, 1] = 255
+        got = product(kind, **args)
+        nan = torch.isnan(got)
+        want = torch.zeros_like(nan)
+        want[:, n - 3] = True
+        if kind == "gemm":
+            want[m - 2] = True
+        assert torch.equal(nan, want) and torch.equal(got[~nan], first[~nan])
 
 
 @pytest.mark.parametrize("pad", [1, 3, 8])
