@@ -148,7 +148,8 @@ int mv_op_quantize_mxfp4(void* stream, int32_t N, int32_t K, int32_t dtype, cons
                          void* dequantised);
 /* out[M][N] = x . W^T + bias, with codes2 / scales2 the gated pair silu(x . W^T + bias) * (x . W2^T + bias2); then + residual.  x bf16 [M][ldx];
  * W, W2 MXFP4 [N][K]; bias, bias2 bf16 [N] or NULL; residual [M][N] of the output's type or NULL (may be `out` itself); out_dtype MV_BF16 or
- * MV_F32.  The weights enter the matrix cores as bf16 (exact), sums are fp32, the result is rounded once. */
+ * MV_F32.  The weights enter the matrix cores as bf16 (exact), sums are fp32, the result is rounded once.  The kernel is chosen by the sizes, so a
+ * row's last bits may differ between calls of different M; equal calls give equal bits. */
 int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x, int64_t ldx, const void* codes, const void* scales,
                        const void* codes2, const void* scales2, const void* bias, const void* bias2, const void* residual, int32_t out_dtype,
                        void* out);
@@ -165,7 +166,7 @@ typedef struct mv_logit_controls {
     const float* presence;       /* [rows] subtracted once from tokens that occur behind the prompt                      */
     const float* frequency;      /* [rows] subtracted once per occurrence behind the prompt                              */
     const int32_t* history;      /* [rows][ld_history] token ids, prompt first; ids outside the vocabulary are ignored   */
-    const int32_t* history_len;  /* [rows] ids in use, clamped to 0 .. history_cap; NULL: history_cap                    */
+    const int32_t* history_len;  /* [rows] ids in use, clamped to 0 .. history_cap (all of which is read); NULL: history_cap */
     const int32_t* prompt_len;   /* [rows] how many of them are the prompt; NULL: 0                                      */
     int64_t ld_history;
     int32_t history_cap;

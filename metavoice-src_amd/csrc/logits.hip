@@ -219,6 +219,8 @@ extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, i
     if (!logits || !out) return mv_fail(MV_ERR_INVALID, "logit_controls: null argument");
     const size_t ein = dtype == MV_F32 ? 4 : 2, eout = out_dtype == MV_F32 ? 4 : 2;
     if (!op_aligned(logits, ein) || !op_aligned(uncond, ein) || !op_aligned(out, eout)) return mv_fail(MV_ERR_INVALID, "logit_controls: a buffer is not aligned to its element");
+    if ((out == logits || out == uncond) && (dtype != out_dtype || ld != ld_out))
+        return mv_fail(MV_ERR_INVALID, "logit_controls: out on top of its input needs the input's dtype and stride");
     if (c.history_cap == 0 || (!c.repetition && !c.presence && !c.frequency)) c.history = nullptr;
     if (c.n_bias == 0) c.bias_ids = nullptr;
     a.chunks = (uint32_t)((vocab + (int64_t)LC_CHUNK - 1) / LC_CHUNK);

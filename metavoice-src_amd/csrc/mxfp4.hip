@@ -837,13 +837,14 @@ hipError_t launch_products(hipStream_t s, MxArgs a, bool x4) {
 }
 
 // the checks that both products share; null: fine
-const char* product_fault(int32_t M, int32_t N, int32_t K, const void* codes, const void* scales, const void* codes2, const void* scales2, const void* bias,
+const char* product_fault(int32_t M, int32_t N, int32_t K, const void* x, const void* codes, const void* scales, const void* codes2, const void* scales2, const void* bias,
                           const void* bias2, const void* residual, int32_t out_dtype, const void* out) {
     if (M < 0 || N < 0 || K < 1) return "M and N must not be negative, K must be positive";
     if (std::max({M, N, K}) > 0x7FFFFFFF - 4096) return "M, N or K is too large";
     if (out_dtype != MV_BF16 && out_dtype != MV_F32) return "out_dtype must be MV_BF16 or MV_F32";
     if (M == 0 || N == 0) return nullptr;
     if (!codes || !scales || !out) return "null argument";
+    if (out == x) return "out on top of x";
     if (!codes2 != !scales2) return "codes2 and scales2 go together";
     if (bias2 && !codes2) return "bias2 without codes2";
     if (!op_aligned(codes, 16) || !op_aligned(codes2, 16)) return "codes must be aligned to 16 bytes";
@@ -892,7 +893,7 @@ int mv_op_quantize_mxfp4(void* stream, int32_t N, int32_t K, int32_t dtype, cons
 
 int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x, int64_t ldx, const void* codes, const void* scales, const void* codes2,
                        const void* scales2, const void* bias, const void* bias2, const void* residual, int32_t out_dtype, void* out) {
-    const char* fault = product_fault(M, N, K, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out);
+    const char* fault = product_fault(M, N, K, x, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out);
     if (!fault && ldx < K) fault = "ldx below K";
     if (!fault && M > 0 && N > 0 && (!x || !op_aligned(x, 2))) fault = "x is null or not aligned to its element";
     if (fault) return mv_fail(MV_ERR_INVALID, "linear_mxfp4: %s (M=%d N=%d K=%d)", fault, M, N, K);
@@ -907,7 +908,7 @@ int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void
 
 int mv_op_gemm_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x_codes, const void* x_scales, const void* codes, const void* scales,
                      const void* codes2, const void* scales2, const void* bias, const void* bias2, const void* residual, int32_t out_dtype, void* out) {
-    const char* fault = product_fault(M, N, K, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out);
+    const char* fault = product_fault(M, N, K, x_codes, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out);
     if (!fault && M > 0 && N > 0 && (!x_codes || !x_scales || !op_aligned(x_codes, 16))) fault = "x_codes must be aligned to 16 bytes, x_scales not null";
     if (fault) return mv_fail(MV_ERR_INVALID, "gemm_mxfp4: %s (M=%d N=%d K=%d)", fault, M, N, K);
     if (M == 0 || N == 0) return MV_OK;

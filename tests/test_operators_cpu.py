@@ -37,17 +37,17 @@ def test_quantize_refuses(kw, text):
     refused(quantize(**kw), text)
 
 
-def linear(m=4, n=8, k=64, x=A, ldx=64, codes=A, scales=A, codes2=None, scales2=None, bias=None, bias2=None, residual=None, out_dtype=0, out=A):
+def linear(m=4, n=8, k=64, x=A, ldx=64, codes=A, scales=A, codes2=None, scales2=None, bias=None, bias2=None, residual=None, out_dtype=0, out=2 * A):
     return N.lib().mv_op_linear_mxfp4(None, m, n, k, x, ldx, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out)
 
 
-def gemm(m=4, n=8, k=64, x=A, xs=A, codes=A, scales=A, codes2=None, scales2=None, bias=None, bias2=None, residual=None, out_dtype=0, out=A):
+def gemm(m=4, n=8, k=64, x=A, xs=A, codes=A, scales=A, codes2=None, scales2=None, bias=None, bias2=None, residual=None, out_dtype=0, out=2 * A):
     return N.lib().mv_op_gemm_mxfp4(None, m, n, k, x, xs, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out)
 
 
 @pytest.mark.parametrize("fn", [linear, gemm])
 @pytest.mark.parametrize("kw,text", [(dict(m=-1), "negative"), (dict(n=-1), "negative"), (dict(k=0), "positive"), (dict(k=-5), "positive"),
-                                     (dict(m=2 ** 31 - 1), "too large"), (dict(n=2 ** 31 - 1), "too large"),
+                                     (dict(out=A), "on top"), (dict(m=2 ** 31 - 1), "too large"), (dict(n=2 ** 31 - 1), "too large"),
                                      (dict(out_dtype=2), "out_dtype"), (dict(codes=None), "null"), (dict(scales=None), "null"), (dict(out=None), "null"),
                                      (dict(x=None), "x"), (dict(codes2=A), "together"), (dict(scales2=A), "together"), (dict(bias2=A), "bias2"),
                                      (dict(codes=A + 4), "16 bytes"), (dict(codes2=A + 4, scales2=A), "16 bytes"), (dict(out=A + 1), "element"),
@@ -63,14 +63,15 @@ def test_products_refuse_their_own():
     refused(gemm(xs=None), "x_scales")
 
 
-def controls(rows=2, vocab=64, dtype=0, logits=A, uncond=None, ld=64, out_dtype=0, out=A, ld_out=64, allowed=None, null=False, **c):
+def controls(rows=2, vocab=64, dtype=0, logits=A, uncond=None, ld=64, out_dtype=0, out=2 * A, ld_out=64, allowed=None, null=False, **c):
     s = N.mv_logit_controls(**c)
     return N.lib().mv_op_logit_controls(None, rows, vocab, dtype, logits, uncond, ld, None if null else s, out_dtype, out, ld_out, allowed)
 
 
 @pytest.mark.parametrize("kw,text", [(dict(rows=-1), "shape"), (dict(vocab=0), "shape"), (dict(dtype=2), "dtype"), (dict(out_dtype=3), "dtype"), (dict(ld=63), "stride"),
                                      (dict(ld_out=63), "stride"), (dict(null=True), "null"), (dict(logits=None), "null"), (dict(out=None), "null"),
-                                     (dict(uncond=A), "guidance"), (dict(history=A, history_cap=8, ld_history=7), "ld_history"), (dict(history_cap=8), "history_cap"),
+                                     (dict(uncond=A), "guidance"), (dict(out=A, out_dtype=1), "on top"), (dict(out=A, ld_out=65), "on top"),
+                                     (dict(uncond=3 * A, guidance=A, out=3 * A, ld_out=65), "on top"), (dict(history=A, history_cap=8, ld_history=7), "ld_history"), (dict(history_cap=8), "history_cap"),
                                      (dict(history_cap=-1), "negative"), (dict(n_bias=-1), "negative"), (dict(n_masks=-1), "negative"),
                                      (dict(bias_ids=A, n_bias=3), "go together"), (dict(bias=A, n_bias=3), "go together"), (dict(n_bias=3), "go together"),
                                      (dict(bias_ids=A, bias=A, n_bias=3, ld_bias=2), "ld_bias"), (dict(mask_index=A), "masks"), (dict(n_masks=2), "masks"),
