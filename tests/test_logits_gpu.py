@@ -161,6 +161,30 @@ def test_masks_row_by_row():
     check(torch.randn(4, v, generator=g).cuda(), None, d, BF)
 
 
+@pytest.fixture
+def room():
+    """Hands back what a test of large buffers took."""
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_offsets_past_32_bits(room):
+    """20000 rows of 131072 tokens: the first and last rows against 64 bits."""
+    rows, v = 20000, 131072
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(rows, v, device="cuda")
+    d = controls(rows, v, g, 40, 5, 3)
+    out, allowed = hip(x, None, d, BF)
+    pick = torch.tensor([0, rows // 2, rows - 1])
+    host = {k: (t if k == "masks" else t[pick.to(t.device)]).cpu().numpy() for k, t in d.items()}
+    host["masks"] = host["masks"].view(np.uint32)
+    want, n, size = o_lg.controls(x[pick.cuda()].cpu().double().numpy(), **host)
+    got = out[pick.cuda()].cpu().double().numpy()
+    fine = np.isfinite(want)
+    assert np.array_equal(allowed[pick.cuda()].cpu().numpy(), n) and np.array_equal(got[~fine], want[~fine])
+    assert (np.abs(got[fine] - want[fine]) <= (8 * 2.0 ** -24 * size + 2.0 ** -8 * np.abs(want))[fine]).all()
+
+
 def test_no_rows():
     y = torch.full((2, 8), 7.0, device="cuda")
     N.check(N.lib().mv_op_logit_controls(stream(), 0, 8, 1, None, None, 8, struct({}), 1, ptr(y), 8, None))

@@ -337,3 +337,92 @@ def test_products_on_two_streams_and_in_a_graph():
         eager = chain(new, bufs())
         torch.cuda.synchronize()
         assert torch.equal(gb[3], eager)
+
+
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+@pytest.mark.parametrize("m,n,k", [(5, 33, 95), (70, 300, 640), (1100, 1300, 640), (2300, 3900, 416)])
+def test_buffers_at_odd_elements(kind, m, n, k):
+    """Everything but the codes may begin at any element: outputs, residuals, biases, bf16 rows, scale bytes."""
+    args, want, size = case(kind, m, n, k, False, True, True, torch.bfloat16, make=make_fast)
+
+    def shift(t, dtype):
+        room = torch.empty(t.numel() + 1, dtype=dtype, device="cuda")
+        room[1:] = t.reshape(-1)
+        return room[1:].view(t.shape)
+
+    args["w"] = (args["w"][0], shift(args["w"][1], torch.uint8))
+    args["bias"], args["residual"] = shift(args["bias"], torch.bfloat16), shift(args["residual"], torch.bfloat16)
+    if kind == "linear":
+        args["x"] = shift(args["x"].contiguous(), torch.bfloat16)
+    else:
+        args["x"] = (args["x"][0], shift(args["x"][1], torch.uint8))
+    room = torch.full((m * n + 2,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = room[1:m * n + 1]
+    act = (ptr(args["x"]), k) if kind == "linear" else (ptr(args["x"][0]), ptr(args["x"][1]))
+    fn = N.lib().mv_op_linear_mxfp4 if kind == "linear" else N.lib().mv_op_gemm_mxfp4
+    N.check(fn(stream(), m, n, k, *act, ptr(args["w"][0]), ptr(args["w"][1]), None, None, ptr(args["bias"]), None, ptr(args["residual"]), 0, ptr(out)))
+    torch.cuda.synchronize()
+    assert float(room[0]) == 7 and float(room[-1]) == 7
+    within(out.view(m, n), want, size, k, torch.bfloat16)
+
+
+@pytest.mark.parametrize("m", [3, 70, 1100, 2300])
+def test_infinities_and_nan_in_x_stay_in_their_rows(m):
+    n, k = 1300 if m < 2000 else 3900, 429
+    args, _, _ = case("linear", m, n, k, False, False, False, torch.float32, make=make_fast)
+    first = product("linear", **args)
+    args["x"] = args["x"].clone()
+    args["x"][m - 1, k - 1], args["x"][0, 0] = float("nan"), float("inf")
+    got = product("linear", **args)
+    assert not bool(torch.isfinite(got[m - 1]).any()) and not bool(torch.isfinite(got[0]).all())
+    assert torch.equal(got[1: m - 1], first[1: m - 1])
+
+
+def codes_on_the_gpu(g, rows, k):
+    nb = o_mx.blocks(k)
+    assert k % 32 == 0
+    return (torch.randint(0, 256, (rows, 16 * nb), generator=g, device="cuda", dtype=torch.uint8),
+            torch.randint(120, 127, (rows, nb), generator=g, device="cuda", dtype=torch.uint8))
+
+
+def host(c):
+    return c[0].cpu().numpy(), c[1].cpu().numpy()
+
+
+def rows_of(c, pick):
+    return c[0][pick].contiguous(), c[1][pick].contiguous()
+
+
+@pytest.fixture
+def room():
+    """Hands back what a test of large buffers took."""
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind,m,n,k", [("linear", 270000, 16, 8192), ("linear", 140000, 16384, 32), ("gemm", 140000, 16384, 64), ("linear", 2, 600000, 16384),
+                                        ("gemm", 300, 600000, 16384), ("gemm", 1100000, 8, 8192)])
+def test_offsets_past_32_bits(kind, m, n, k, room):
+    """x, weights or output of more than 2^31 elements or 2^32 bytes: the last rows and columns against 64 bits."""
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    w = codes_on_the_gpu(g, n, k)
+    x = codes_on_the_gpu(g, m, k) if kind == "gemm" else torch.randn(m, k, generator=g, device="cuda", dtype=torch.bfloat16)
+    out = torch.full((m, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    act = (ptr(x), k) if kind == "linear" else (ptr(x[0]), ptr(x[1]))
+    fn = N.lib().mv_op_linear_mxfp4 if kind == "linear" else N.lib().mv_op_gemm_mxfp4
+    N.check(fn(stream(), m, n, k, *act, ptr(w[0]), ptr(w[1]), None, None, None, None, None, 0, ptr(out)))
+    torch.cuda.synchronize()
+    rows = torch.unique(torch.tensor([0, m // 2, max(0, m - 2), m - 1])).cuda()
+    cols = torch.unique(torch.tensor([0, n // 2, n - 3, n - 1])).cuda()
+    x64 = bits64(x[rows]) if kind == "linear" else o_mx.values(*host(rows_of(x, rows)), k)
+    want, size = o_mx.product(x64, o_mx.values(*host(rows_of(w, cols)), k))
+    within(out[rows][:, cols], want, size, k, torch.bfloat16)
+    assert int((out == 7).sum()) < 0.05 * m * n  # no part was left out
+
+
+def test_quantiser_offsets_past_32_bits(room):
+    rows, k = 300000, 8192
+    w = torch.randn(rows, k, device="cuda", dtype=torch.bfloat16)
+    codes, scales, deq = hip_quantize(w)
+    for lo in (0, rows // 2, rows - 50):
+        check_quantised(w[lo:lo + 50], codes[lo:lo + 50], scales[lo:lo + 50], deq[lo:lo + 50])
