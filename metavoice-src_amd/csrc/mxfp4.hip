@@ -22,6 +22,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));    // 16 bytes at the alignment of a bf16 element
 typedef f32x4_t f32x4_any __attribute__((aligned(4)));  // and of a float
+typedef uint64_t u64_byte __attribute__((aligned(1)));
 
 #define MX_TRY(expr)                                                                                                               \
     do {                                                                                                                           \
@@ -185,6 +186,7 @@ __device__ __forceinline__ void mx_store8(const MxArgs& a, int m, int n, float (
 __device__ __forceinline__ u32x4 mx_load_x8(const bf16_t* row, int c, int K) {
     if (c + 8 <= K) return *(const u32x4_any*)(row + c);
     u32x4 r = {0u, 0u, 0u, 0u};
+    if (c >= K) return r;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (c + i < K) r[i >> 1] |= (uint32_t)row[c + i] << (16 * (i & 1));
@@ -203,16 +205,40 @@ __device__ __forceinline__ bf16x8_t mx_widen(uint32_t q, float scale) {
 #define MX_INLINE __attribute__((always_inline))
 #define MX_WAVES 8
 
-// Few rows: one workgroup computes 16 MT rows of x against 16 NT weight rows; its waves take the 128-column steps of K in turn, each straight from memory
-// to registers, and their sums meet in LDS, in wave order.  Lane (r = lane & 15, g = lane >> 4) holds block 4 step + g of weight row r and of x row
-// r: the weights are the first operand of the matrix instruction, so a lane ends with 4 consecutive output columns of one row.  Bound by what a CU reads
-// (about 30 bytes per nanosecond of x and weights), or by latency when the matrix is small.
+// Few rows: one workgroup computes 16 MT rows of x against 16 NT weight rows; its waves take the 256-column steps of K in turn, each straight from memory
+// to registers, and their sums meet in LDS, in wave order.  The weights are the first operand of the matrix instruction, so a lane ends with 4
+// consecutive output columns of one row.  Bound by the cache lines that a CU reads, or by latency when the matrix is small.
+// A load of a wave covers 8 rows x 128 bytes, whole lines: lane (r = lane & 15, g = lane >> 4) reads row r & 7 (a second load: 8 + (r & 7)), piece
+// g + 4 (r >> 3) of 16 bytes.  mx_pair turns two such loads into the two halves of the 128 bytes in operand order: row r, pieces g and 4 + g.
+__device__ __forceinline__ void mx_pair(u32x4& a, u32x4& b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // rotated by 8 within 16 lanes; lanes 8 .. 15 of the first, 0 .. 7 of the second half
+        const uint32_t p = a[i], q = b[i];
+        a[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)p, (int)q, 0x128, 0xF, 0xC, false);
+        b[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)q, (int)p, 0x128, 0xF, 0x3, false);
+    }
+}
+// lane group g holds the four words of block g -> word j of the result holds word g of block j
+__device__ __forceinline__ u32x4 mx_across(const u32x4& w) {
+    const auto p = __builtin_amdgcn_permlane16_swap(w[0], w[1], false, false), q = __builtin_amdgcn_permlane16_swap(w[2], w[3], false, false);
+    const auto e = __builtin_amdgcn_permlane32_swap(p[0], q[0], false, false), o = __builtin_amdgcn_permlane32_swap(p[1], q[1], false, false);
+    return u32x4{(uint32_t)e[0], (uint32_t)o[0], (uint32_t)e[1], (uint32_t)o[1]};
+}
+// the scales of 8 blocks of a row; past its end anything but 255 will do, the codes there are zeros
+__device__ __forceinline__ uint64_t mx_scales8(const unsigned char* row, int b, int nb) {
+    if (b + 8 <= nb) return *(const u64_byte*)(row + b);
+    if (nb >= 8) return *(const u64_byte*)(row + nb - 8) >> (8 * (b + 8 - nb));
+    uint64_t s = 0;
+    for (int i = b; i < nb; ++i) s |= (uint64_t)row[i] << (8 * (i - b));
+    return s;
+}
+
 template <bool X4, bool GATED, int MT, int NT>
 __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs a) {
-    constexpr int MATS = GATED ? 2 : 1, XW = X4 ? 1 : 4;  // 16-byte pieces of an x row per step
+    constexpr int MATS = GATED ? 2 : 1, XQ = X4 ? 1 : 4;  // 128-byte pieces of an x row per step
     extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [wave][matrix, weight tile, x tile][lane]
     constexpr int TILES = MATS * NT * MT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, piece = g + 4 * (r >> 3);
     const uint32_t tm = blockIdx.x / a.tiles_n, tn = blockIdx.x - tm * a.tiles_n;
     const int m0 = (int)tm * 16 * MT, n0 = (int)tn * 16 * NT;
     f32x4_t acc[MATS][NT][MT];
@@ -222,70 +248,78 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int m = 0; m < MT; ++m) acc[i][n][m] = f32x4_t{0, 0, 0, 0};
-    for (int b0 = wave * 4; b0 < a.nb; b0 += MX_WAVES * 4) {
-        const int b = b0 + g;
-        const bool in_k = b < a.nb;
-        u32x4 wq[MATS][NT], xq[MT][XW];
-        uint32_t wsc[MATS][NT], xsc[MT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int row = n0 + n * 16 + r;
-            const bool in = in_k && row < a.N;
-            const int64_t at = (int64_t)row * a.nb + b;
-#pragma unroll
-            for (int i = 0; i < MATS; ++i) {
-                wq[i][n] = u32x4{0u, 0u, 0u, 0u};
-                wsc[i][n] = 127u;
-                if (in) {
-                    wq[i][n] = *(const u32x4*)((i ? a.w2 : a.w) + at * 16);
-                    wsc[i][n] = (i ? a.ws2 : a.ws)[at];
-                }
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const int row = m0 + m * 16 + r;
-            const bool in = in_k && row < a.M;
-            xsc[m] = 127u;
-#pragma unroll
-            for (int j = 0; j < XW; ++j) xq[m][j] = u32x4{0u, 0u, 0u, 0u};
-            if (in) {
-                if (X4) {
-                    const int64_t at = (int64_t)row * a.nb + b;
-                    xq[m][0] = *(const u32x4*)((const unsigned char*)a.x + at * 16);
-                    xsc[m] = a.xs[at];
-                } else {
-                    const bf16_t* p = (const bf16_t*)a.x + (int64_t)row * a.ldx;
-                    if (b * 32 + 32 <= a.K) {
-#pragma unroll
-                        for (int j = 0; j < XW; ++j) xq[m][j] = *(const u32x4_any*)(p + b * 32 + j * 8);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < XW; ++j) xq[m][j] = mx_load_x8(p, b * 32 + j * 8, a.K);
-                    }
-                }
-            }
-        }
+    for (int b0 = wave * 8; b0 < a.nb; b0 += MX_WAVES * 8) {
+        u32x4 w[MATS][NT][2], x[MT][XQ][2];
+        uint64_t ws[MATS][NT], xs[MT];
+        const bool in_k = b0 + piece < a.nb;
 #pragma unroll
         for (int i = 0; i < MATS; ++i)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const u32x4 w = wq[i][n];
-                if (X4) {
-                    const i32x8_t wv = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) {
-                        const u32x4 x = xq[m][0];
-                        const i32x8_t xv = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
-                        acc[i][n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i][n][m], 4, 4, 0, (int)wsc[i][n], 0, (int)xsc[m]);
+                for (int e = 0; e < 2; ++e) {
+                    const int row = n0 + n * 16 + e * 8 + (r & 7);
+                    w[i][n][e] = u32x4{0u, 0u, 0u, 0u};
+                    if (in_k && row < a.N) w[i][n][e] = *(const u32x4*)((i ? a.w2 : a.w) + ((int64_t)row * a.nb + b0 + piece) * 16);
+                }
+                const int row = min(n0 + n * 16 + r, a.N - 1);
+                ws[i][n] = mx_scales8((i ? a.ws2 : a.ws) + (int64_t)row * a.nb, b0, a.nb);
+            }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = m0 + m * 16 + e * 8 + (r & 7);
+#pragma unroll
+                for (int q = 0; q < XQ; ++q) x[m][q][e] = u32x4{0u, 0u, 0u, 0u};
+                if (row < a.M) {
+                    if (X4) {
+                        if (in_k) x[m][0][e] = *(const u32x4*)((const unsigned char*)a.x + ((int64_t)row * a.nb + b0 + piece) * 16);
+                    } else {
+                        const bf16_t* p = (const bf16_t*)a.x + (int64_t)row * a.ldx;
+                        if (b0 * 32 + 256 <= a.K) {
+#pragma unroll
+                            for (int q = 0; q < XQ; ++q) x[m][q][e] = *(const u32x4_any*)(p + b0 * 32 + q * 64 + piece * 8);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < XQ; ++q) x[m][q][e] = mx_load_x8(p, b0 * 32 + q * 64 + piece * 8, a.K);
+                        }
                     }
-                } else {
+                }
+            }
+            if (X4) xs[m] = mx_scales8(a.xs + (int64_t)min(m0 + m * 16 + r, a.M - 1) * a.nb, b0, a.nb);
+        }
 #pragma unroll
-                    for (int j = 0; j < XW; ++j) {
-                        const bf16x8_t wv = mx_widen(w[j], __uint_as_float(wsc[i][n] << 23));
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-                        for (int m = 0; m < MT; ++m)
-                            acc[i][n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, xq[m][j]), acc[i][n][m], 0, 0, 0);
+            for (int q = 0; q < XQ; ++q) mx_pair(x[m][q][0], x[m][q][1]);
+#pragma unroll
+        for (int i = 0; i < MATS; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mx_pair(w[i][n][0], w[i][n][1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {  // blocks b0 + 4 e + ..
+                    const uint32_t sw = (uint32_t)(ws[i][n] >> (32 * e));
+                    if (X4) {
+                        const u32x4 v = w[i][n][e];
+                        const i32x8_t wv = {(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            const u32x4 u = x[m][0][e];
+                            const i32x8_t xv = {(int)u[0], (int)u[1], (int)u[2], (int)u[3], 0, 0, 0, 0};
+                            acc[i][n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i][n][m], 4, 4, 0, (int)(sw >> (8 * g)), 0,
+                                                                                           (int)((uint32_t)(xs[m] >> (32 * e)) >> (8 * g)));
+                        }
+                    } else {  // x piece 8 q + 4 e' + g is part g of block 2 q + e'
+                        const u32x4 v = mx_across(w[i][n][e]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const bf16x8_t wv = mx_widen(v[j], __uint_as_float(((sw >> (8 * j)) & 255u) << 23));
+#pragma unroll
+                            for (int m = 0; m < MT; ++m)
+                                acc[i][n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, x[m][(4 * e + j) >> 1 & (XQ - 1)][j & 1]), acc[i][n][m], 0, 0, 0);
+                        }
                     }
                 }
             }
@@ -799,27 +833,31 @@ hipError_t launch_rows(hipStream_t s, MxArgs a) {
     return hipGetLastError();
 }
 
-// Estimated microseconds of the two kernels, in the coefficients that a fit to 180 measured products gives (1 .. 2048 rows, 100 .. 16384 columns, K from
+// Estimated microseconds of the two kernels, in the coefficients that a fit to 198 measured products gives (1 .. 2048 rows, 100 .. 16384 columns, K from
 // 300 to 8192; the choice by them costs 2 - 3 % over the best one on average).  A workgroup of the first kernel reads its rows of x and of the
 // weights; what counts is how much a CU reads.  One of the second advances by stages, a little slower when all CUs work.
 template <bool X4>
 double rows_us(const MxArgs& a, int mt, int nt) {
     const double mats = a.w2 ? 2 : 1, wgs = (double)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt));
     const double kb = 1e-3 * a.nb * (std::min(a.M, 16 * mt) * (X4 ? 17 : 64) + 16 * nt * mats * 17);
-    return (X4 ? 2.5 : 2.9) + (X4 ? 0.155 : 0.26) * mt * nt * mats + (X4 ? 0.046 : 0.034) * kb * std::max(1.0, wgs / 256);
+    return (X4 ? 2.7 : 3.4) + (X4 ? 0.156 : 0.276) * mt * nt * mats + kb * (X4 ? 0.0353 * std::max(1.0, wgs / 256) + 0.0048 * std::min(1.0, wgs / 256)
+                                                                             : 0.0313 * std::max(1.0, wgs / 256) + 0.0015 * std::min(1.0, wgs / 256));
 }
 template <bool X4>
 double tiles_us(const MxArgs& a, int edge) {
     const double tiles = (double)((a.M + edge - 1) / edge) * (((a.w2 ? 2.0 : 1.0) * a.N + edge - 1) / edge), rounds = std::ceil(tiles / 256);
     const double full = std::min(1.0, tiles / 256), blocks = a.nb;
-    if (edge == 128) return X4 ? 2.1 + rounds * (3.0 + blocks * (0.056 + 0.049 * full)) : 2.3 + rounds * (3.8 + blocks * (0.168 + 0.1 * full));
-    return X4 ? 7.0 + rounds * blocks * (0.176 + 0.144 * full) : 10.4 + rounds * (blocks * (0.54 + 0.3 * full) - 0.9);
+    if (edge == 128) return X4 ? 2.5 + rounds * (3.1 + blocks * (0.049 + 0.05 * full)) : 4.1 + rounds * (2.3 + blocks * (0.172 + 0.105 * full));
+    return X4 ? 6.1 + rounds * (1.6 + blocks * (0.168 + 0.117 * full)) : 9.3 + rounds * (0.3 + blocks * (0.564 + 0.238 * full));
 }
 
 template <bool X4, bool GATED>
 hipError_t choose(hipStream_t s, const MxArgs& a) {
-    const double r11 = rows_us<X4>(a, 1, 1), r12 = rows_us<X4>(a, 1, 2), r14 = rows_us<X4>(a, 1, 4), r22 = rows_us<X4>(a, 2, 2), r24 = rows_us<X4>(a, 2, 4);
-    const double rows = std::min({r11, r12, r14, r22, r24});
+    // Tiles of the first kernel in 16s of rows and columns.  With bf16 rows more columns come before more rows, since a row costs what 4 columns do; two
+    // matrices of 2 x 4 do not fit the registers.
+    constexpr int M3 = X4 ? 2 : 1, N3 = X4 ? 2 : 4, N4 = GATED ? 2 : 4;
+    const double r1 = rows_us<X4>(a, 1, 1), r2 = rows_us<X4>(a, 1, 2), r3 = rows_us<X4>(a, M3, N3), r4 = rows_us<X4>(a, 2, N4);
+    const double rows = std::min({r1, r2, r3, r4});
     const int64_t x_row = X4 ? (int64_t)a.nb * 16 : a.ldx * 2;
     // the second kernel counts bytes within a workgroup's rows, and workgroups, in 32 bits
     if (x_row <= 1 << 23 && a.nb <= 1 << 19 && (double)a.M * a.N < 1e13) {
@@ -827,11 +865,10 @@ hipError_t choose(hipStream_t s, const MxArgs& a) {
         if (a.x_direct && t256 < t128 && t256 < rows) return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
         if (t128 < rows) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
     }
-    if (r11 == rows) return launch_rows<X4, GATED, 1, 1>(s, a);
-    if (r12 == rows) return launch_rows<X4, GATED, 1, 2>(s, a);
-    if (r14 == rows) return launch_rows<X4, GATED, 1, 4>(s, a);
-    if (r22 == rows) return launch_rows<X4, GATED, 2, 2>(s, a);
-    return launch_rows<X4, GATED, 2, 4>(s, a);
+    if (r1 == rows) return launch_rows<X4, GATED, 1, 1>(s, a);
+    if (r2 == rows) return launch_rows<X4, GATED, 1, 2>(s, a);
+    if (r3 == rows) return launch_rows<X4, GATED, M3, N3>(s, a);
+    return launch_rows<X4, GATED, 2, N4>(s, a);
 }
 
 hipError_t launch_products(hipStream_t s, MxArgs a, bool x4) {
