@@ -205,11 +205,15 @@ __device__ __forceinline__ bf16x8_t mx_widen(uint32_t q, float scale) {
 #define MX_INLINE __attribute__((always_inline))
 #define MX_WAVES 8
 
-// Few rows: one workgroup computes 16 MT rows of x against 16 NT weight rows; its waves take the 256-column steps of K in turn, each straight from memory
-// to registers, and their sums meet in LDS, in wave order.  The weights are the first operand of the matrix instruction, so a lane ends with 4
-// consecutive output columns of one row.  Bound by the cache lines that a CU reads, or by latency when the matrix is small.
-// A load of a wave covers 8 rows x 128 bytes, whole lines: lane (r = lane & 15, g = lane >> 4) reads row r & 7 (a second load: 8 + (r & 7)), piece
-// g + 4 (r >> 3) of 16 bytes.  mx_pair turns two such loads into the two halves of the 128 bytes in operand order: row r, pieces g and 4 + g.
+// Few rows: one workgroup computes 16 MT rows of x against 16 NT weight rows; its waves take steps of K in turn, each straight from memory to registers,
+// and their sums meet in LDS, in wave order.  The weights are the first operand of the matrix instruction, so a lane ends with 4 consecutive output
+// columns of one row.  Bound by the cache lines that a CU reads, or by latency when the matrix is small.
+// LINES, where all rows begin on a 128-byte line: a step is 256 columns and a load of a wave covers 8 rows x 128 bytes.  Lane (r = lane & 15, g =
+// lane >> 4) reads row r & 7 (a second load: 8 + (r & 7)), piece g + 4 (r >> 3) of 16 bytes; mx_pair turns two such loads into the two halves of the
+// 128 bytes in operand order: row r, pieces g and 4 + g.
+// Without it a step is 128 columns and the lane reads block g of row r, which is its operand already.  On whole lines the first is 5 - 8 % faster with
+// bf16 rows and 10 - 25 % with codes (16 x 16384 x 8192: 25.3 -> 23.2 us, 21.6 -> 18.3 us); on rows that straddle lines it loses 10 - 25 % (16 x 4096 x
+// 4064: 5.8 -> 6.3 us, 4.4 -> 5.0 us).
 __device__ __forceinline__ void mx_pair(u32x4& a, u32x4& b) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // rotated by 8 within 16 lanes; lanes 8 .. 15 of the first, 0 .. 7 of the second half
@@ -224,21 +228,19 @@ __device__ __forceinline__ u32x4 mx_across(const u32x4& w) {
     const auto e = __builtin_amdgcn_permlane32_swap(p[0], q[0], false, false), o = __builtin_amdgcn_permlane32_swap(p[1], q[1], false, false);
     return u32x4{(uint32_t)e[0], (uint32_t)o[0], (uint32_t)e[1], (uint32_t)o[1]};
 }
-// the scales of 8 blocks of a row; past its end anything but 255 will do, the codes there are zeros
-__device__ __forceinline__ uint64_t mx_scales8(const unsigned char* row, int b, int nb) {
-    if (b + 8 <= nb) return *(const u64_byte*)(row + b);
-    if (nb >= 8) return *(const u64_byte*)(row + nb - 8) >> (8 * (b + 8 - nb));
-    uint64_t s = 0;
-    for (int i = b; i < nb; ++i) s |= (uint64_t)row[i] << (8 * (i - b));
-    return s;
+// the scales of a step: 8 of a row, or one; past the row's end anything but 255 will do, the codes there are zeros
+template <bool LINES>
+__device__ __forceinline__ uint64_t mx_row_scales(const unsigned char* row, int b0, int g, int nb) {
+    if constexpr (LINES) return *(const u64_byte*)(row + b0);  // 8 at a time: nb is a multiple of 8
+    else return b0 + g < nb ? row[b0 + g] : 127u;
 }
 
-template <bool X4, bool GATED, int MT, int NT>
+template <bool X4, bool GATED, bool LINES, int MT, int NT>
 __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs a) {
-    constexpr int MATS = GATED ? 2 : 1, XQ = X4 ? 1 : 4;  // 128-byte pieces of an x row per step
+    constexpr int MATS = GATED ? 2 : 1, XQ = X4 ? 1 : 4, E = LINES ? 2 : 1, STEP = 4 * E;  // blocks per step
     extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [wave][matrix, weight tile, x tile][lane]
     constexpr int TILES = MATS * NT * MT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, piece = g + 4 * (r >> 3);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, piece = LINES ? g + 4 * (r >> 3) : g;
     const uint32_t tm = blockIdx.x / a.tiles_n, tn = blockIdx.x - tm * a.tiles_n;
     const int m0 = (int)tm * 16 * MT, n0 = (int)tn * 16 * NT;
     f32x4_t acc[MATS][NT][MT];
@@ -248,28 +250,31 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int m = 0; m < MT; ++m) acc[i][n][m] = f32x4_t{0, 0, 0, 0};
-    for (int b0 = wave * 8; b0 < a.nb; b0 += MX_WAVES * 8) {
-        u32x4 w[MATS][NT][2], x[MT][XQ][2];
-        uint64_t ws[MATS][NT], xs[MT];
+    for (int b0 = wave * STEP; b0 < a.nb; b0 += MX_WAVES * STEP) {
+        u32x4 w[MATS][NT][E], x[MT][XQ][E];
+        uint64_t ws[MATS][NT], xs[MT];  // LINES: the step's 8 scales of row r; else block g's own
         const bool in_k = b0 + piece < a.nb;
 #pragma unroll
-        for (int i = 0; i < MATS; ++i)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int e = 0; e < E; ++e) {
+                const int row = n0 + n * 16 + (LINES ? e * 8 + (r & 7) : r);
+                const int64_t at = ((int64_t)row * a.nb + b0 + piece) * 16;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = n0 + n * 16 + e * 8 + (r & 7);
-                    w[i][n][e] = u32x4{0u, 0u, 0u, 0u};
-                    if (in_k && row < a.N) w[i][n][e] = *(const u32x4*)((i ? a.w2 : a.w) + ((int64_t)row * a.nb + b0 + piece) * 16);
-                }
-                const int row = min(n0 + n * 16 + r, a.N - 1);
-                ws[i][n] = mx_scales8((i ? a.ws2 : a.ws) + (int64_t)row * a.nb, b0, a.nb);
+                for (int i = 0; i < MATS; ++i) w[i][n][e] = u32x4{0u, 0u, 0u, 0u};
+                if (in_k && row < a.N)
+#pragma unroll
+                    for (int i = 0; i < MATS; ++i) w[i][n][e] = *(const u32x4*)((i ? a.w2 : a.w) + at);
             }
+            const int64_t row = (int64_t)min(n0 + n * 16 + r, a.N - 1) * a.nb;
+#pragma unroll
+            for (int i = 0; i < MATS; ++i) ws[i][n] = mx_row_scales<LINES>((i ? a.ws2 : a.ws) + row, b0, g, a.nb);
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = m0 + m * 16 + e * 8 + (r & 7);
+            for (int e = 0; e < E; ++e) {
+                const int row = m0 + m * 16 + (LINES ? e * 8 + (r & 7) : r);
 #pragma unroll
                 for (int q = 0; q < XQ; ++q) x[m][q][e] = u32x4{0u, 0u, 0u, 0u};
                 if (row < a.M) {
@@ -277,29 +282,35 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
                         if (in_k) x[m][0][e] = *(const u32x4*)((const unsigned char*)a.x + ((int64_t)row * a.nb + b0 + piece) * 16);
                     } else {
                         const bf16_t* p = (const bf16_t*)a.x + (int64_t)row * a.ldx;
-                        if (b0 * 32 + 256 <= a.K) {
+                        const int c = b0 * 32 + piece * (LINES ? 8 : 32);  // the pieces of 8 columns: 64 apart, or a block's four
+                        if (LINES ? (b0 + STEP) * 32 <= a.K : c + 32 <= a.K) {
 #pragma unroll
-                            for (int q = 0; q < XQ; ++q) x[m][q][e] = *(const u32x4_any*)(p + b0 * 32 + q * 64 + piece * 8);
-                        } else {
+                            for (int q = 0; q < XQ; ++q) x[m][q][e] = *(const u32x4_any*)(p + c + q * (LINES ? 64 : 8));
+                        } else if (LINES || in_k) {
 #pragma unroll
-                            for (int q = 0; q < XQ; ++q) x[m][q][e] = mx_load_x8(p, b0 * 32 + q * 64 + piece * 8, a.K);
+                            for (int q = 0; q < XQ; ++q) x[m][q][e] = mx_load_x8(p, c + q * (LINES ? 64 : 8), a.K);
                         }
                     }
                 }
             }
-            if (X4) xs[m] = mx_scales8(a.xs + (int64_t)min(m0 + m * 16 + r, a.M - 1) * a.nb, b0, a.nb);
+            if (X4) xs[m] = mx_row_scales<LINES>(a.xs + (int64_t)min(m0 + m * 16 + r, a.M - 1) * a.nb, b0, g, a.nb);
         }
+        if constexpr (LINES) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int q = 0; q < XQ; ++q) mx_pair(x[m][q][0], x[m][q][1]);
+                for (int q = 0; q < XQ; ++q) mx_pair(x[m][q][0], x[m][q][E - 1]);
+#pragma unroll
+            for (int i = 0; i < MATS; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mx_pair(w[i][n][0], w[i][n][E - 1]);
+        }
 #pragma unroll
         for (int i = 0; i < MATS; ++i)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mx_pair(w[i][n][0], w[i][n][1]);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {  // blocks b0 + 4 e + ..
+                for (int e = 0; e < E; ++e) {  // blocks b0 + 4 e + ..
                     const uint32_t sw = (uint32_t)(ws[i][n] >> (32 * e));
                     if (X4) {
                         const u32x4 v = w[i][n][e];
@@ -308,21 +319,23 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
                         for (int m = 0; m < MT; ++m) {
                             const u32x4 u = x[m][0][e];
                             const i32x8_t xv = {(int)u[0], (int)u[1], (int)u[2], (int)u[3], 0, 0, 0, 0};
-                            acc[i][n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i][n][m], 4, 4, 0, (int)(sw >> (8 * g)), 0,
-                                                                                           (int)((uint32_t)(xs[m] >> (32 * e)) >> (8 * g)));
+                            const uint32_t sx = (uint32_t)(xs[m] >> (32 * e));
+                            acc[i][n][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i][n][m], 4, 4, 0, (int)(LINES ? sw >> (8 * g) : sw), 0,
+                                                                                           (int)(LINES ? sx >> (8 * g) : sx));
                         }
-                    } else {  // x piece 8 q + 4 e' + g is part g of block 2 q + e'
-                        const u32x4 v = mx_across(w[i][n][e]);
+                    } else {  // LINES: x piece 8 q + 4 e' + g is part g of block 2 q + e'; else lane group g has part j of its block at turn j
+                        const u32x4 v = LINES ? mx_across(w[i][n][e]) : w[i][n][e];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const bf16x8_t wv = mx_widen(v[j], __uint_as_float(((sw >> (8 * j)) & 255u) << 23));
+                            const uint32_t s = LINES ? sw >> (8 * j) & 255u : sw;
+                            const bf16x8_t wv = mx_widen(v[j], __uint_as_float(s << 23));
 #pragma unroll
                             for (int m = 0; m < MT; ++m)
-                                acc[i][n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, __builtin_bit_cast(bf16x8_t, x[m][(4 * e + j) >> 1 & (XQ - 1)][j & 1]), acc[i][n][m], 0, 0, 0);
+                                acc[i][n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    wv, __builtin_bit_cast(bf16x8_t, LINES ? x[m][(4 * e + j) >> 1 & (XQ - 1)][j & (E - 1)] : x[m][j & (XQ - 1)][0]), acc[i][n][m], 0, 0, 0);
                         }
                     }
                 }
-            }
     }
 #pragma unroll
     for (int i = 0; i < MATS; ++i)
@@ -811,10 +824,10 @@ hipError_t launch_tiles(hipStream_t s, MxArgs a) {
     return hipGetLastError();
 }
 
-template <bool X4, bool GATED, int MT, int NT>
+template <bool X4, bool GATED, bool LINES, int MT, int NT>
 hipError_t launch_rows(hipStream_t s, MxArgs a) {
     constexpr int LDS = MX_WAVES * (GATED ? 2 : 1) * MT * NT * 1024;
-    constexpr auto kernel = mx_rows_kernel<X4, GATED, MT, NT>;
+    constexpr auto kernel = mx_rows_kernel<X4, GATED, LINES, MT, NT>;
     const hipError_t e = LDS > 64 * 1024 ? allow_lds<kernel>(LDS) : hipSuccess;
     if (e != hipSuccess) return e;
     a.tiles_n = (uint32_t)((a.N + 16 * NT - 1) / (16 * NT));
@@ -833,25 +846,25 @@ hipError_t launch_rows(hipStream_t s, MxArgs a) {
     return hipGetLastError();
 }
 
-// Estimated microseconds of the two kernels, in the coefficients that a fit to 198 measured products gives (1 .. 2048 rows, 100 .. 16384 columns, K from
-// 300 to 8192; the choice by them costs 2 - 3 % over the best one on average).  A workgroup of the first kernel reads its rows of x and of the
-// weights; what counts is how much a CU reads.  One of the second advances by stages, a little slower when all CUs work.
+// Estimated microseconds of the two kernels, in the coefficients that a fit to 255 sets of measured products gives (1 .. 2048 rows, 100 .. 16384 columns,
+// K from 300 to 8192; the choice by them costs 1 - 2 % over the best one on average).  A workgroup of the first kernel reads its rows of x and of the
+// weights; what counts is how much the busiest CU reads (workgroups with 4 and more products share one unevenly: rounds of them count).  One of the
+// second advances by stages, a little slower when all CUs work.
 template <bool X4>
 double rows_us(const MxArgs& a, int mt, int nt) {
-    const double mats = a.w2 ? 2 : 1, wgs = (double)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt));
-    const double kb = 1e-3 * a.nb * (std::min(a.M, 16 * mt) * (X4 ? 17 : 64) + 16 * nt * mats * 17);
-    return (X4 ? 2.7 : 3.4) + (X4 ? 0.156 : 0.276) * mt * nt * mats + kb * (X4 ? 0.0353 * std::max(1.0, wgs / 256) + 0.0048 * std::min(1.0, wgs / 256)
-                                                                             : 0.0313 * std::max(1.0, wgs / 256) + 0.0015 * std::min(1.0, wgs / 256));
+    const double mats = a.w2 ? 2 : 1, products = mt * nt * mats, per_cu = (double)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt)) / 256;
+    const double kb = 1e-3 * a.nb * (std::min(a.M, 16 * mt) * (X4 ? 17 : 64) + 16 * nt * mats * 17), times = products < 4 ? std::max(1.0, per_cu) : std::ceil(per_cu);
+    return X4 ? 2.4 + 0.16 * products + 0.037 * kb * times : 2.9 + 0.245 * products + 0.033 * kb * times;
 }
 template <bool X4>
 double tiles_us(const MxArgs& a, int edge) {
-    const double tiles = (double)((a.M + edge - 1) / edge) * (((a.w2 ? 2.0 : 1.0) * a.N + edge - 1) / edge), rounds = std::ceil(tiles / 256);
+    const double tiles = (double)((a.M + edge - 1) / edge) * (((a.w2 ? 2ll : 1ll) * a.N + edge - 1) / edge), rounds = std::ceil(tiles / 256);
     const double full = std::min(1.0, tiles / 256), blocks = a.nb;
-    if (edge == 128) return X4 ? 2.5 + rounds * (3.1 + blocks * (0.049 + 0.05 * full)) : 4.1 + rounds * (2.3 + blocks * (0.172 + 0.105 * full));
-    return X4 ? 6.1 + rounds * (1.6 + blocks * (0.168 + 0.117 * full)) : 9.3 + rounds * (0.3 + blocks * (0.564 + 0.238 * full));
+    if (edge == 128) return X4 ? 2.2 + rounds * (3.4 + blocks * (0.049 + 0.045 * full)) : 3.2 + rounds * (4.1 + blocks * (0.172 + 0.072 * full));
+    return X4 ? 7.5 + rounds * blocks * (0.164 + 0.138 * full) : 10.8 + rounds * (blocks * (0.557 + 0.267 * full) - 1.4);
 }
 
-template <bool X4, bool GATED>
+template <bool X4, bool GATED, bool LINES>
 hipError_t choose(hipStream_t s, const MxArgs& a) {
     // Tiles of the first kernel in 16s of rows and columns.  With bf16 rows more columns come before more rows, since a row costs what 4 columns do; two
     // matrices of 2 x 4 do not fit the registers.
@@ -865,16 +878,18 @@ hipError_t choose(hipStream_t s, const MxArgs& a) {
         if (a.x_direct && t256 < t128 && t256 < rows) return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
         if (t128 < rows) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
     }
-    if (r1 == rows) return launch_rows<X4, GATED, 1, 1>(s, a);
-    if (r2 == rows) return launch_rows<X4, GATED, 1, 2>(s, a);
-    if (r3 == rows) return launch_rows<X4, GATED, M3, N3>(s, a);
-    return launch_rows<X4, GATED, 2, N4>(s, a);
+    if (r1 == rows) return launch_rows<X4, GATED, LINES, 1, 1>(s, a);
+    if (r2 == rows) return launch_rows<X4, GATED, LINES, 1, 2>(s, a);
+    if (r3 == rows) return launch_rows<X4, GATED, LINES, M3, N3>(s, a);
+    return launch_rows<X4, GATED, LINES, 2, N4>(s, a);
 }
 
 hipError_t launch_products(hipStream_t s, MxArgs a, bool x4) {
     a.x_direct = x4 || (op_aligned(a.x, 4) && a.ldx % 2 == 0);
     a.s_direct = a.nb % 4 == 0 && op_aligned(a.ws, 4) && op_aligned(a.ws2, 4) && op_aligned(a.xs, 4);
-    return x4 ? (a.w2 ? choose<true, true>(s, a) : choose<true, false>(s, a)) : (a.w2 ? choose<false, true>(s, a) : choose<false, false>(s, a));
+    const bool lines = a.nb % 8 == 0 && op_aligned(a.w, 128) && op_aligned(a.w2, 128) && op_aligned(a.x, 128) && (x4 || a.ldx % 64 == 0);
+    if (lines) return x4 ? (a.w2 ? choose<true, true, true>(s, a) : choose<true, false, true>(s, a)) : (a.w2 ? choose<false, true, true>(s, a) : choose<false, false, true>(s, a));
+    return x4 ? (a.w2 ? choose<true, true, false>(s, a) : choose<true, false, false>(s, a)) : (a.w2 ? choose<false, true, false>(s, a) : choose<false, false, false>(s, a));
 }
 
 // the checks that both products share; null: fine

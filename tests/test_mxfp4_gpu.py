@@ -176,10 +176,12 @@ def test_product(kind, m, n, k):
 
 
 # Products large enough for the row kernels of several tiles and for both tiled kernels: whole and short stages, rows of scales that are and are not
-# aligned (ceil(K / 32) a multiple of 4 or not), ragged last tiles, an odd number of stages.
+# aligned (ceil(K / 32) a multiple of 4 or not), rows that begin on a cache line (a multiple of 8) and that do not, ragged last tiles, an odd number of
+# stages.
 LARGE = [(25, 6000, 1500), (30, 9000, 600), (700, 900, 1088), (600, 1500, 1100), (1100, 1300, 640), (1537, 4100, 320), (2049, 4100, 200), (1300, 6200, 1000),
          (1100, 8300, 225), (2300, 3900, 289), (513, 2500, 2049), (3000, 3100, 1024),
-         (90, 1900, 1130), (88, 3700, 1116), (112, 10078, 517), (88, 4010, 2100)]
+         (90, 1900, 1130), (88, 3700, 1116), (112, 10078, 517), (88, 4010, 2100),
+         (18, 8049, 1280), (36, 8191, 1024), (74, 6529, 1280), (67, 6273, 955)]
 
 
 @pytest.mark.parametrize("m,n,k", LARGE)
