@@ -138,8 +138,8 @@ int mv_op_attention_rows(void* stream, int32_t batch, int32_t T, int32_t n_head,
  * Format: a row of K values in nb = ceil(K / 32) blocks of 32 columns; a block is 32 codes of 4 bits (sign, 2 exponent bits, 1 mantissa bit:
  * 0 0.5 1 1.5 2 3 4 6) times 2^(s - 127), s its scale byte; s = 255: NaN.
  *   codes  [rows][16 nb] bytes (column 2j low, 2j + 1 high nibble of byte j; zero past K), 16-byte aligned;   scales [rows][nb] bytes
- * A call with no row or no column (M, N or rows 0) does nothing.  Sizes and strides count elements; strides need no alignment, but 16-byte
- * aligned rows are read fastest.
+ * A call with no row or no column (M, N or rows 0) does nothing.  Sizes and strides count elements; strides need no alignment, but rows that
+ * begin on 128 bytes (K a multiple of 256) are read fastest.  Outputs lie apart from inputs except where a call says otherwise.
  *
  * mv_op_quantize_mxfp4: w [N][ldw], dtype MV_BF16 or MV_F32 -> codes, scales and, when not NULL, the values they stand for as bf16 [N][K]
  * (`dequantised` may be w itself when w is bf16 and ldw = K).  Block exponent floor(log2 max|w|) - 2, at least -127; codes rounded to nearest,

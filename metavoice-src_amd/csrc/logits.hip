@@ -16,6 +16,8 @@
 #include "common.h"
 #include "op_common.h"
 
+#include <algorithm>
+
 #define LC_THREADS 512
 #define LC_GROUPS 2                                // groups of 4 consecutive tokens per thread
 #define LC_CHUNK (LC_THREADS * LC_GROUPS * 4)      // 4096 tokens: two words each are 32 KB of LDS
@@ -40,7 +42,7 @@ struct ControlArgs {
     int32_t* allowed;
     int64_t ld, ld_out;
     int32_t vocab;
-    uint32_t chunks, groups;  // chunks of a row, and its workgroups: one more where the mask's bits are counted
+    uint32_t rows, chunks, groups;  // chunks of a row, and its workgroups: one more where the mask's bits are counted
 };
 
 // 4 consecutive logits of a row from token v on, zero past the vocabulary
@@ -74,7 +76,8 @@ __global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const Contro
     __shared__ __attribute__((aligned(16))) uint32_t entry[LC_CHUNK];  // 1 + the bias entry that holds, 0: none
     const mv_logit_controls& c = a.c;
     const int tid = threadIdx.x;
-    const uint32_t row = blockIdx.x / a.groups, chunk = blockIdx.x - row * a.groups;
+    const uint32_t id = op_workgroup(), row = id / a.groups, chunk = id - row * a.groups;
+    if (row >= a.rows) return;
     const int index = c.masks == nullptr ? -1 : c.mask_index ? c.mask_index[row] : (int)row;
     const uint32_t* mask = index >= 0 && index < c.n_masks ? c.masks + (int64_t)index * c.ld_mask : nullptr;
 
@@ -205,10 +208,11 @@ extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, i
         return mv_fail(MV_ERR_INVALID, "logit_controls: dtype %d -> %d (MV_BF16 or MV_F32)", dtype, out_dtype);
     if (ld < vocab || ld_out < vocab) return mv_fail(MV_ERR_INVALID, "logit_controls: a row stride (%lld, %lld) is below the vocabulary %d", (long long)ld, (long long)ld_out, vocab);
     if (!controls) return mv_fail(MV_ERR_INVALID, "logit_controls: null argument");
-    ControlArgs a{*controls, logits, uncond, out, allowed, ld, ld_out, vocab, 0, 0};
+    ControlArgs a{*controls, logits, uncond, out, allowed, ld, ld_out, vocab, (uint32_t)rows, 0, 0};
     mv_logit_controls& c = a.c;
     if (uncond && !c.guidance) return mv_fail(MV_ERR_INVALID, "logit_controls: uncond without guidance");
     if (c.history_cap < 0 || c.n_bias < 0 || c.n_masks < 0) return mv_fail(MV_ERR_INVALID, "logit_controls: a negative count");
+    if (std::max({vocab, c.history_cap, c.n_bias}) > 0x7FFFFFFF - LC_CHUNK) return mv_fail(MV_ERR_INVALID, "logit_controls: vocab, history_cap or n_bias is too large");
     if (c.history && c.ld_history < c.history_cap) return mv_fail(MV_ERR_INVALID, "logit_controls: ld_history below history_cap");
     if (!c.history && c.history_cap) return mv_fail(MV_ERR_INVALID, "logit_controls: history_cap without history");
     if (!c.bias_ids != !c.bias || (!c.bias && c.n_bias)) return mv_fail(MV_ERR_INVALID, "logit_controls: bias_ids, bias and n_bias go together");
@@ -220,6 +224,9 @@ extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, i
     if (!logits || !out) return mv_fail(MV_ERR_INVALID, "logit_controls: null argument");
     const size_t ein = dtype == MV_F32 ? 4 : 2, eout = out_dtype == MV_F32 ? 4 : 2;
     if (!op_aligned(logits, ein) || !op_aligned(uncond, ein) || !op_aligned(out, eout)) return mv_fail(MV_ERR_INVALID, "logit_controls: a buffer is not aligned to its element");
+    for (const void* p : {(const void*)c.guidance, (const void*)c.repetition, (const void*)c.presence, (const void*)c.frequency, (const void*)c.history, (const void*)c.history_len,
+                          (const void*)c.prompt_len, (const void*)c.bias_ids, (const void*)c.bias, (const void*)c.masks, (const void*)c.mask_index, (const void*)allowed})
+        if (!op_aligned(p, 4)) return mv_fail(MV_ERR_INVALID, "logit_controls: a buffer is not aligned to its element");
     if ((out == logits || out == uncond) && (dtype != out_dtype || ld != ld_out))
         return mv_fail(MV_ERR_INVALID, "logit_controls: out on top of its input needs the input's dtype and stride");
     if (c.history_cap == 0 || (!c.repetition && !c.presence && !c.frequency)) c.history = nullptr;
@@ -229,7 +236,7 @@ extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, i
     if ((int64_t)a.groups * rows > 0x7FFFFFFF) return mv_fail(MV_ERR_INVALID, "logit_controls: rows=%d vocab=%d is too large", rows, vocab);
     OpDevice dev((hipStream_t)stream, out);
     LC_TRY(dev.status());
-    const dim3 grid(a.groups * (uint32_t)rows), block(LC_THREADS);
+    const dim3 grid = op_grid((uint64_t)a.groups * rows), block(LC_THREADS);
     if (dtype == MV_F32 && out_dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<true, true>), grid, block, 0, (hipStream_t)stream, a);
     else if (dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<true, false>), grid, block, 0, (hipStream_t)stream, a);
     else if (out_dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<false, true>), grid, block, 0, (hipStream_t)stream, a);

@@ -243,7 +243,8 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
     extern __shared__ __attribute__((aligned(16))) f32x4_t part[];  // [wave][matrix, weight tile, x tile][lane]
     constexpr int TILES = MATS * NT * MT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4, piece = LINES ? g + 4 * (r >> 3) : g;
-    const uint32_t tm = blockIdx.x / a.tiles_n, tn = blockIdx.x - tm * a.tiles_n;
+    const uint32_t id = op_workgroup(), tm = id / a.tiles_n, tn = id - tm * a.tiles_n;
+    if (tm * (16 * MT) >= (uint32_t)a.M) return;
     const int m0 = (int)tm * 16 * MT, n0 = (int)tn * 16 * NT;
     f32x4_t acc[MATS][NT][MT];
 #pragma unroll
@@ -837,18 +838,8 @@ hipError_t launch_rows(hipStream_t s, MxArgs a) {
     const hipError_t e = LDS > 64 * 1024 ? allow_lds<kernel>(LDS) : hipSuccess;
     if (e != hipSuccess) return e;
     a.tiles_n = (uint32_t)((a.N + 16 * NT - 1) / (16 * NT));
-    const int64_t rows_per_launch = std::max<int64_t>(1, 0x7FFFFFFF / (int64_t)a.tiles_n / (16 * MT)) * (16 * MT);  // a grid is below 2^31 workgroups
-    const int M = a.M;
-    const int64_t x_row = X4 ? (int64_t)a.nb * 16 : a.ldx * 2, y_row = (int64_t)a.N * (a.out_f32 ? 4 : 2);
-    for (int64_t m0 = 0; m0 < M; m0 += rows_per_launch) {
-        MxArgs b = a;
-        b.M = (int)std::min<int64_t>(M - m0, rows_per_launch);
-        b.x = (const char*)a.x + m0 * x_row;
-        if (X4) b.xs = a.xs + m0 * a.nb;
-        if (a.res) b.res = (const char*)a.res + m0 * y_row;
-        b.out = (char*)a.out + m0 * y_row;
-        hipLaunchKernelGGL(kernel, dim3(a.tiles_n * (uint32_t)((b.M + 16 * MT - 1) / (16 * MT))), dim3(64 * MX_WAVES), LDS, s, b);
-    }
+    const uint64_t tiles_m = (uint32_t)((a.M + 16 * MT - 1) / (16 * MT));
+    hipLaunchKernelGGL(kernel, op_grid(tiles_m * a.tiles_n), dim3(64 * MX_WAVES), LDS, s, a);
     return hipGetLastError();
 }
 
@@ -878,8 +869,8 @@ hipError_t choose(hipStream_t s, const MxArgs& a) {
     const double r1 = rows_us<X4>(a, 1, 1), r2 = rows_us<X4>(a, 1, 2), r3 = rows_us<X4>(a, M3, N3), r4 = rows_us<X4>(a, 2, N4);
     const double rows = std::min({r1, r2, r3, r4});
     const int64_t x_row = X4 ? (int64_t)a.nb * 16 : a.ldx * 2;
-    // the second kernel counts bytes within a workgroup's rows, and workgroups, in 32 bits
-    if (x_row <= 1 << 23 && a.nb <= 1 << 19 && (double)a.M * a.N < 1e13) {
+    // the second kernel counts bytes within a workgroup's rows in 32 bits, and its threads are one dimension of a grid
+    if (x_row <= 1 << 23 && a.nb <= 1 << 19 && ((a.M + 127ll) / 128) * ((a.N * (GATED ? 2ll : 1ll) + 127) / 128) < 1 << OP_GRID_BITS) {
         const double t128 = tiles_us<X4>(a, 128), t256 = tiles_us<X4>(a, 256);
         if (a.x_direct && t256 < t128 && t256 < rows) return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
         if (t128 < rows) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
@@ -928,6 +919,8 @@ int mv_op_quantize_mxfp4(void* stream, int32_t N, int32_t K, int32_t dtype, cons
     const size_t esz = dtype == MV_F32 ? 4 : 2;
     if (!op_aligned(w, esz) || !op_aligned(codes, 16) || !op_aligned(dequantised, 2))
         return mv_fail(MV_ERR_INVALID, "quantize_mxfp4: codes must be aligned to 16 bytes, the other buffers to their element");
+    if (codes == w || scales == w || (dequantised == w && (dtype != MV_BF16 || ldw != K)))
+        return mv_fail(MV_ERR_INVALID, "quantize_mxfp4: an output on top of w (dequantised may be, with bf16 and ldw = K)");
     OpDevice dev((hipStream_t)stream, codes);
     MX_TRY(dev.status());
     QuantArgs a;

@@ -44,6 +44,15 @@ class OpDevice {
     hipError_t status_ = hipSuccess;
 };
 
+// n workgroups of up to 512 threads.  A grid's dimension is below 2^32 threads: beyond 2^22 workgroups a second one counts on, and the last workgroups
+// find nothing to do.
+constexpr int OP_GRID_BITS = 22;
+inline dim3 op_grid(uint64_t n) {
+    if (n <= 1u << OP_GRID_BITS) return dim3((uint32_t)n);
+    return dim3(1u << OP_GRID_BITS, (uint32_t)((n + (1u << OP_GRID_BITS) - 1) >> OP_GRID_BITS));
+}
+__device__ __forceinline__ uint32_t op_workgroup() { return blockIdx.y << OP_GRID_BITS | blockIdx.x; }
+
 inline bool op_aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 // n / d for 0 <= n < 2^31 by a multiply and a shift

@@ -185,6 +185,19 @@ def test_offsets_past_32_bits(room):
     assert (np.abs(got[fine] - want[fine]) <= (8 * 2.0 ** -24 * size + 2.0 ** -8 * np.abs(want))[fine]).all()
 
 
+def test_more_workgroups_than_one_grid_dimension_takes(room):
+    """Nine million rows of three tokens, two workgroups each: biases of one shared list and one of two masks are exact."""
+    rows, v = 9000000, 3
+    x = torch.randint(-50, 50, (rows, v), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).float()
+    d = dict(bias_ids=torch.tensor([[2, 0]], dtype=torch.int32, device="cuda"), bias=torch.tensor([[4.0, -8.0]], device="cuda"),
+             masks=torch.tensor([[0b111], [0b101]], dtype=torch.int32, device="cuda"), mask_index=(torch.arange(rows, device="cuda") % 2).int())
+    got, n = hip(x, None, d, F)
+    want = x + torch.tensor([-8.0, 0.0, 4.0], device="cuda")
+    want[1::2, 1] = -float("inf")
+    assert torch.equal(got, want)
+    assert torch.equal(n, 3 - d["mask_index"])
+
+
 def test_no_rows():
     y = torch.full((2, 8), 7.0, device="cuda")
     N.check(N.lib().mv_op_logit_controls(stream(), 0, 8, 1, None, None, 8, struct({}), 1, ptr(y), 8, None))

@@ -429,3 +429,37 @@ def test_quantiser_offsets_past_32_bits(room):
     codes, scales, deq = hip_quantize(w)
     for lo in (0, rows // 2, rows - 50):
         check_quantised(w[lo:lo + 50], codes[lo:lo + 50], scales[lo:lo + 50], deq[lo:lo + 50])
+
+
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+@pytest.mark.parametrize("m,n", [(140000000, 1), (1, 140000000)])
+def test_more_workgroups_than_one_grid_dimension_takes(kind, m, n, room):
+    """8.75 million workgroups of 512 threads; two columns of K, so a result is a sum of two products: at most three fp32 half steps of their magnitudes
+    (2^-24 each), then the output's own half step, 2^-8."""
+    g = torch.Generator(device="cuda").manual_seed(m % 1000 + n % 1000)
+    k = 2
+
+    def two(rows):  # codes of the first two columns, zeros behind them; scale 1
+        b = torch.zeros(rows, 16, dtype=torch.uint8, device="cuda")
+        b[:, 0] = torch.randint(0, 256, (rows,), generator=g, device="cuda", dtype=torch.uint8)
+        return b, torch.full((rows, 1), 127, dtype=torch.uint8, device="cuda")
+
+    def values(c):
+        table = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, 0, -.5, -1, -1.5, -2, -3, -4, -6], device="cuda")
+        return torch.stack([table[(c[0][:, 0] & 15).int()], table[(c[0][:, 0] >> 4).int()]], 1)
+
+    w = two(n)
+    x = two(m) if kind == "gemm" else torch.randn(m, k, generator=g, device="cuda", dtype=torch.bfloat16)
+    out = torch.full((m, n), 7.5, dtype=torch.bfloat16, device="cuda")
+    act = (ptr(x), k) if kind == "linear" else (ptr(x[0]), ptr(x[1]))
+    fn = N.lib().mv_op_linear_mxfp4 if kind == "linear" else N.lib().mv_op_gemm_mxfp4
+    N.check(fn(stream(), m, n, k, *act, ptr(w[0]), ptr(w[1]), None, None, None, None, None, 0, ptr(out)))
+    torch.cuda.synchronize()
+    long, short = (x, w) if m > n else (w, x)
+    short = (values(short) if isinstance(short, tuple) else short).double()
+    out = out.view(-1)
+    for lo in range(0, max(m, n), 20000000):
+        part = tuple(t[lo:lo + 20000000] for t in long) if isinstance(long, tuple) else long[lo:lo + 20000000]
+        terms = (values(part) if isinstance(part, tuple) else part).double() * short
+        want, size = terms.sum(1), terms.abs().sum(1)
+        assert bool(((out[lo:lo + 20000000].double() - want).abs() <= 3 * 2.0 ** -24 * size + 2.0 ** -8 * want.abs()).all()), lo

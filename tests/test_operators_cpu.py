@@ -32,7 +32,9 @@ def quantize(n=4, k=64, dtype=0, w=A, ldw=64, codes=A, scales=A, deq=None):
 @pytest.mark.parametrize("kw,text", [(dict(n=-1), "shape"), (dict(k=0), "shape"), (dict(k=2 ** 31 - 1, ldw=2 ** 40), "shape"), (dict(dtype=2), "dtype"),
                                      (dict(dtype=3), "dtype"), (dict(ldw=63), "ldw"), (dict(ldw=-64), "ldw"), (dict(w=None), "null"), (dict(codes=None), "null"),
                                      (dict(scales=None), "null"), (dict(codes=A + 8), "aligned"), (dict(w=A + 1), "aligned"),
-                                     (dict(w=A + 2, dtype=1), "aligned"), (dict(deq=A + 1), "aligned")])
+                                     (dict(w=A + 2, dtype=1), "aligned"), (dict(deq=A + 1), "aligned"), (dict(), "on top"),
+                                     (dict(codes=2 * A), "on top"), (dict(codes=2 * A, scales=3 * A, deq=A, dtype=1), "on top"),
+                                     (dict(codes=2 * A, scales=3 * A, deq=A, ldw=65), "on top")])
 def test_quantize_refuses(kw, text):
     refused(quantize(**kw), text)
 
@@ -77,6 +79,10 @@ def controls(rows=2, vocab=64, dtype=0, logits=A, uncond=None, ld=64, out_dtype=
                                      (dict(bias_ids=A, bias=A, n_bias=3, ld_bias=2), "ld_bias"), (dict(mask_index=A), "masks"), (dict(n_masks=2), "masks"),
                                      (dict(masks=A, n_masks=2, ld_mask=1), "ld_mask"), (dict(masks=A, n_masks=1, ld_mask=2), "mask_index"),
                                      (dict(logits=A + 1), "aligned"), (dict(out=A + 2, out_dtype=1), "aligned"), (dict(uncond=A + 1, guidance=A), "aligned"),
+                                     (dict(guidance=A + 2), "aligned"), (dict(history=A + 1, history_cap=8, ld_history=8), "aligned"), (dict(allowed=A + 2), "aligned"),
+                                     (dict(masks=A + 2, n_masks=2, ld_mask=2), "aligned"), (dict(vocab=2 ** 31 - 1, ld=2 ** 31, ld_out=2 ** 31), "too large"),
+                                     (dict(history=A, history_cap=2 ** 31 - 1, ld_history=2 ** 31), "too large"),
+                                     (dict(bias_ids=A, bias=A, n_bias=2 ** 31 - 1), "too large"),
                                      (dict(rows=2 ** 31 - 1, vocab=8193, ld=8193, ld_out=8193), "too large")])
 def test_controls_refuse(kw, text):
     refused(controls(**kw), text)
