@@ -375,7 +375,9 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
 // codes do).
 // LDS has 64 banks and serves 16 lanes of a 16-byte read at a time: chunk c of a row lies at c ^ (row / (rows per 256 bytes)), so 16 rows
 // spread over all banks.  A transfer writes LDS in lane order: the permutation is applied to the lane's address in memory.
-// Two tiles: 256 x 256 (8 waves of 64 rows x 128 columns), and 128 x 128 whose two teams of 4 waves split a stage's columns, for grids that leave CUs idle.
+// Four tiles, the smaller ones for grids that would leave CUs idle, their waves in teams that split a stage's columns: 256 x 256 (8 waves of 64 rows x 128
+// columns), 128 x 128 and 64 x 128 (two teams of 4 waves), 64 x 64 (bf16 rows: four teams of 2, codes: two of 4).  64 x 16384 x 8192 by the last one: bf16
+// rows 27 us (the 128 tile: 57), codes 15 us (24), the weights at 4.7 TB/s.
 // Measured: bf16 rows 4096 x 16384 x 8192 in 840 us, 1.31 PFLOP/s (a library product of two bf16 matrices: 704 us); codes 8192 x 16384 x 8192 in 560 us, 3.9
 // PFLOP/s; 256 x 5632 x 2048 gated 11 us.  Bound by power: the matrix units are busy 68 % (bf16) and 57 % (codes) of the time at 1.8 GHz, and a loop of the
 // same matrix instructions alone, on the same data in registers, takes 685 us and 2 x 216 us.
@@ -843,42 +845,45 @@ hipError_t launch_rows(hipStream_t s, MxArgs a) {
     return hipGetLastError();
 }
 
-// Estimated microseconds of the two kernels, in the coefficients that a fit to 255 sets of measured products gives (1 .. 2048 rows, 100 .. 16384 columns,
-// K from 300 to 8192; the choice by them costs 1 - 2 % over the best one on average).  A workgroup of the first kernel reads its rows of x and of the
-// weights; what counts is how much the busiest CU reads (workgroups with 4 and more products share one unevenly: rounds of them count).  One of the
-// second advances by stages, a little slower when all CUs work.
+// Estimated microseconds of the two kernels, in the coefficients that a fit to 476 sets of measured products gives (1 .. 2048 rows, 100 .. 16384 columns,
+// K from 300 to 11008; the choice by them costs 1 % over the best one on average, and without one of the four tiles 2 - 6 %).  A workgroup of the first
+// kernel reads its rows of x and of the weights; what counts is how much the busiest CU reads (workgroups with 4 and more products share one unevenly:
+// rounds of them count).  One of the second advances by stages, a little slower when all CUs work, 1.4 times as long where scales come through registers.
 template <bool X4>
 double rows_us(const MxArgs& a, int mt, int nt) {
     const double mats = a.w2 ? 2 : 1, products = mt * nt * mats, per_cu = (double)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt)) / 256;
     const double kb = 1e-3 * a.nb * (std::min(a.M, 16 * mt) * (X4 ? 17 : 64) + 16 * nt * mats * 17), times = products < 4 ? std::max(1.0, per_cu) : std::ceil(per_cu);
-    return X4 ? 2.4 + 0.16 * products + 0.037 * kb * times : 2.9 + 0.245 * products + 0.033 * kb * times;
+    return X4 ? 2.5 + 0.152 * products + 0.035 * kb * times : 2.8 + 0.276 * products + 0.031 * kb * times;
 }
-template <bool X4>
-double tiles_us(const MxArgs& a, int edge) {
-    const double tiles = (double)((a.M + edge - 1) / edge) * (((a.w2 ? 2ll : 1ll) * a.N + edge - 1) / edge), rounds = std::ceil(tiles / 256);
-    const double full = std::min(1.0, tiles / 256), blocks = a.nb;
-    if (edge == 128) return X4 ? 2.2 + rounds * (3.4 + blocks * (0.049 + 0.045 * full)) : 3.2 + rounds * (4.1 + blocks * (0.172 + 0.072 * full));
-    return X4 ? 7.5 + rounds * blocks * (0.164 + 0.138 * full) : 10.8 + rounds * (blocks * (0.557 + 0.267 * full) - 1.4);
+struct TileCost { int bm, bn; double call, round, block, full; };
+constexpr TileCost MX_COST[2][4] = {{{64, 64, 2.2, 2.5, 0.064, 0.021}, {64, 128, 2.8, 2.0, 0.111, 0.039}, {128, 128, 2.2, 3.6, 0.173, 0.074}, {256, 256, 8.9, 2.2, 0.481, 0.253}},
+                                    {{64, 64, 2.1, 1.7, 0.026, 0.014}, {64, 128, 2.4, 1.9, 0.035, 0.025}, {128, 128, 2.1, 3.0, 0.053, 0.040}, {256, 256, 5.6, 2.6, 0.146, 0.111}}};
+double tiles_us(const MxArgs& a, const TileCost& c) {
+    const double tiles = (double)((a.M + c.bm - 1) / c.bm) * (((a.w2 ? 2ll : 1ll) * a.N + c.bn - 1) / c.bn), rounds = std::ceil(tiles / 256);
+    return c.call + rounds * (c.round + a.nb * (a.s_direct ? 1.0 : 1.4) * (c.block + c.full * std::min(1.0, tiles / 256)));
 }
 
 template <bool X4, bool GATED, bool LINES>
 hipError_t choose(hipStream_t s, const MxArgs& a) {
-    // Tiles of the first kernel in 16s of rows and columns.  With bf16 rows more columns come before more rows, since a row costs what 4 columns do; two
-    // matrices of 2 x 4 do not fit the registers.
-    constexpr int M3 = X4 ? 2 : 1, N3 = X4 ? 2 : 4, N4 = GATED ? 2 : 4;
-    const double r1 = rows_us<X4>(a, 1, 1), r2 = rows_us<X4>(a, 1, 2), r3 = rows_us<X4>(a, M3, N3), r4 = rows_us<X4>(a, 2, N4);
-    const double rows = std::min({r1, r2, r3, r4});
+    // Tiles of the first kernel in 16s of rows and columns.  With bf16 rows more columns come before more rows, since a row costs what 4 columns do.
+    constexpr int M3 = X4 ? 2 : 1, N3 = X4 ? 2 : 4;
+    const double r1 = rows_us<X4>(a, 1, 1), r2 = rows_us<X4>(a, 1, 2), r3 = rows_us<X4>(a, M3, N3), rows = std::min({r1, r2, r3});
     const int64_t x_row = X4 ? (int64_t)a.nb * 16 : a.ldx * 2;
     // the second kernel counts bytes within a workgroup's rows in 32 bits, and its threads are one dimension of a grid
-    if (x_row <= 1 << 23 && a.nb <= 1 << 19 && ((a.M + 127ll) / 128) * ((a.N * (GATED ? 2ll : 1ll) + 127) / 128) < 1 << OP_GRID_BITS) {
-        const double t128 = tiles_us<X4>(a, 128), t256 = tiles_us<X4>(a, 256);
-        if (a.x_direct && t256 < t128 && t256 < rows) return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
-        if (t128 < rows) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
+    if (x_row <= 1 << 23 && a.nb <= 1 << 19 && ((a.M + 63ll) / 64) * ((a.N * (GATED ? 2ll : 1ll) + 63) / 64) < 1 << OP_GRID_BITS) {
+        const TileCost* c = MX_COST[X4];
+        const double t1 = tiles_us(a, c[0]), t2 = tiles_us(a, c[1]), t3 = tiles_us(a, c[2]), t4 = a.x_direct ? tiles_us(a, c[3]) : 1e30;
+        const double tiles = std::min({t1, t2, t3, t4});
+        if (tiles < rows) {
+            if (t1 == tiles) return launch_tiles<X4, X4 ? 2 : 4, X4 ? 2 : 1, 2, X4 ? 1 : 2, 1, GATED>(s, a);
+            if (t2 == tiles) return launch_tiles<X4, 2, 2, 2, 2, 1, GATED>(s, a);
+            if (t3 == tiles) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
+            return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
+        }
     }
     if (r1 == rows) return launch_rows<X4, GATED, LINES, 1, 1>(s, a);
     if (r2 == rows) return launch_rows<X4, GATED, LINES, 1, 2>(s, a);
-    if (r3 == rows) return launch_rows<X4, GATED, LINES, M3, N3>(s, a);
-    return launch_rows<X4, GATED, LINES, 2, N4>(s, a);
+    return launch_rows<X4, GATED, LINES, M3, N3>(s, a);
 }
 
 hipError_t launch_products(hipStream_t s, MxArgs a, bool x4) {
