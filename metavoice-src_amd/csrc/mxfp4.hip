@@ -375,12 +375,12 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
 // codes do).
 // LDS has 64 banks and serves 16 lanes of a 16-byte read at a time: chunk c of a row lies at c ^ (row / (rows per 256 bytes)), so 16 rows
 // spread over all banks.  A transfer writes LDS in lane order: the permutation is applied to the lane's address in memory.
-// Four tiles, the smaller ones for grids that would leave CUs idle, their waves in teams that split a stage's columns: 256 x 256 (8 waves of 64 rows x 128
-// columns), 128 x 128 and 64 x 128 (two teams of 4 waves), 64 x 64 (bf16 rows: four teams of 2, codes: two of 4).  64 x 16384 x 8192 by the last one: bf16
-// rows 27 us (the 128 tile: 57), codes 15 us (24), the weights at 4.7 TB/s.
-// Measured: bf16 rows 4096 x 16384 x 8192 in 840 us, 1.31 PFLOP/s (a library product of two bf16 matrices: 704 us); codes 8192 x 16384 x 8192 in 560 us, 3.9
-// PFLOP/s; 256 x 5632 x 2048 gated 11 us.  Bound by power: the matrix units are busy 68 % (bf16) and 57 % (codes) of the time at 1.8 GHz, and a loop of the
-// same matrix instructions alone, on the same data in registers, takes 685 us and 2 x 216 us.
+// Five tiles, the smaller ones for grids that would leave CUs idle: 256 x 256 (8 waves of 64 rows x 128 columns) and 128 x 256 (8 of 64 x 64); with the waves
+// in teams that split a stage's columns 128 x 128 and 64 x 128 (two teams of 4 waves) and 64 x 64 (bf16 rows: four teams of 2, codes: two of 4).
+// Measured: 64 x 16384 x 8192 by the last one bf16 rows 27 us (128 x 128: 57), codes 15 us (24), the weights at 4.7 TB/s; 384 x 16384 x 8192 by 128 x 256
+// codes 38 us (47), bf16 rows 108 us (121); by 256 x 256 bf16 rows 4096 x 16384 x 8192 in 840 us, 1.31 PFLOP/s (a library product of two bf16 matrices:
+// 704 us), codes 8192 x 16384 x 8192 in 560 us, 3.9 PFLOP/s.  The last two are bound by power: the matrix units are busy 68 % (bf16) and 57 % (codes) of
+// the time at 1.8 GHz, and a loop of the same matrix instructions alone, on the same data in registers, takes 685 us and 2 x 216 us.
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* glb_ptr_t;
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
         }
     };
     // What transfers cannot bring comes through registers, zeros past K: the short stage at the end of a row, and rows of bf16 that are not aligned to 4
-    // bytes.  The latter are asked for at one stage and put into LDS at the next (the larger tile has no registers for that and does not take them).
+    // bytes.  The latter are asked for at one stage and put into LDS at the next (by the tiles of teams; the largest has no registers for that).
     auto carry_w = [&](int st, int buf) MX_INLINE {
         const int v = st * KS + team;
 #pragma unroll 1
@@ -845,8 +845,8 @@ hipError_t launch_rows(hipStream_t s, MxArgs a) {
     return hipGetLastError();
 }
 
-// Estimated microseconds of the two kernels, in the coefficients that a fit to 476 sets of measured products gives (1 .. 2048 rows, 100 .. 16384 columns,
-// K from 300 to 11008; the choice by them costs 1 % over the best one on average, and without one of the four tiles 2 - 6 %).  A workgroup of the first
+// Estimated microseconds of the two kernels, in the coefficients that a fit to 602 sets of measured products gives (1 .. 2048 rows, 100 .. 16384 columns,
+// K from 300 to 11008; the choice by them costs 1 % over the best one on average, and without one of the five tiles 2 - 7 %).  A workgroup of the first
 // kernel reads its rows of x and of the weights; what counts is how much the busiest CU reads (workgroups with 4 and more products share one unevenly:
 // rounds of them count).  One of the second advances by stages, a little slower when all CUs work, 1.4 times as long where scales come through registers.
 template <bool X4>
@@ -856,8 +856,9 @@ double rows_us(const MxArgs& a, int mt, int nt) {
     return X4 ? 2.5 + 0.152 * products + 0.035 * kb * times : 2.8 + 0.276 * products + 0.031 * kb * times;
 }
 struct TileCost { int bm, bn; double call, round, block, full; };
-constexpr TileCost MX_COST[2][4] = {{{64, 64, 2.2, 2.5, 0.064, 0.021}, {64, 128, 2.8, 2.0, 0.111, 0.039}, {128, 128, 2.2, 3.6, 0.173, 0.074}, {256, 256, 8.9, 2.2, 0.481, 0.253}},
-                                    {{64, 64, 2.1, 1.7, 0.026, 0.014}, {64, 128, 2.4, 1.9, 0.035, 0.025}, {128, 128, 2.1, 3.0, 0.053, 0.040}, {256, 256, 5.6, 2.6, 0.146, 0.111}}};
+constexpr TileCost MX_COST[2][5] = {
+    {{64, 64, 2.2, 2.5, 0.064, 0.021}, {64, 128, 2.8, 2.0, 0.111, 0.039}, {128, 128, 2.2, 3.6, 0.173, 0.074}, {128, 256, 2.4, 3.4, 0.326, 0.111}, {256, 256, 8.9, 2.2, 0.481, 0.253}},
+    {{64, 64, 2.1, 1.7, 0.026, 0.014}, {64, 128, 2.4, 1.9, 0.035, 0.025}, {128, 128, 2.1, 3.0, 0.053, 0.040}, {128, 256, 1.4, 4.2, 0.089, 0.056}, {256, 256, 5.6, 2.6, 0.146, 0.111}}};
 double tiles_us(const MxArgs& a, const TileCost& c) {
     const double tiles = (double)((a.M + c.bm - 1) / c.bm) * (((a.w2 ? 2ll : 1ll) * a.N + c.bn - 1) / c.bn), rounds = std::ceil(tiles / 256);
     return c.call + rounds * (c.round + a.nb * (a.s_direct ? 1.0 : 1.4) * (c.block + c.full * std::min(1.0, tiles / 256)));
@@ -872,12 +873,13 @@ hipError_t choose(hipStream_t s, const MxArgs& a) {
     // the second kernel counts bytes within a workgroup's rows in 32 bits, and its threads are one dimension of a grid
     if (x_row <= 1 << 23 && a.nb <= 1 << 19 && ((a.M + 63ll) / 64) * ((a.N * (GATED ? 2ll : 1ll) + 63) / 64) < 1 << OP_GRID_BITS) {
         const TileCost* c = MX_COST[X4];
-        const double t1 = tiles_us(a, c[0]), t2 = tiles_us(a, c[1]), t3 = tiles_us(a, c[2]), t4 = a.x_direct ? tiles_us(a, c[3]) : 1e30;
-        const double tiles = std::min({t1, t2, t3, t4});
+        const double t1 = tiles_us(a, c[0]), t2 = tiles_us(a, c[1]), t3 = tiles_us(a, c[2]);
+        const double t4 = a.x_direct ? tiles_us(a, c[3]) : 1e30, t5 = a.x_direct ? tiles_us(a, c[4]) : 1e30, tiles = std::min({t1, t2, t3, t4, t5});
         if (tiles < rows) {
             if (t1 == tiles) return launch_tiles<X4, X4 ? 2 : 4, X4 ? 2 : 1, 2, X4 ? 1 : 2, 1, GATED>(s, a);
             if (t2 == tiles) return launch_tiles<X4, 2, 2, 2, 2, 1, GATED>(s, a);
             if (t3 == tiles) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
+            if (t4 == tiles) return launch_tiles<X4, 1, 4, 2, 2, 2, GATED>(s, a);
             return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
         }
     }

@@ -182,7 +182,7 @@ LARGE = [(25, 6000, 1500), (30, 9000, 600), (700, 900, 1088), (600, 1500, 1100),
          (1100, 8300, 225), (2300, 3900, 289), (513, 2500, 2049), (3000, 3100, 1024),
          (90, 1900, 1130), (88, 3700, 1116), (112, 10078, 517), (88, 4010, 2100),
          (18, 8049, 1280), (36, 8191, 1024), (74, 6529, 1280), (67, 6273, 955),
-         (17, 4201, 512), (17, 8151, 1078), (546, 5411, 65), (193, 8603, 256), (18, 41090, 512), (40, 9001, 640), (250, 3000, 2000), (100, 9003, 1110)]
+         (17, 4201, 512), (17, 8151, 1078), (546, 5411, 65), (193, 8603, 256), (18, 41090, 512), (40, 9001, 640), (250, 3000, 2000), (100, 9003, 1110), (227, 8366, 250)]
 
 
 @pytest.mark.parametrize("m,n,k", LARGE)
