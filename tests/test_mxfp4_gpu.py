@@ -175,7 +175,7 @@ def test_product(kind, m, n, k):
         within(product(kind, **args), want, size, k, dtype)
 
 
-# Products large enough for the row kernels of several tiles and for both tiled kernels: whole and short stages, rows of scales that are and are not
+# Products large enough for the row kernels of several tiles and for every tiled kernel: whole and short stages, rows of scales that are and are not
 # aligned (ceil(K / 32) a multiple of 4 or not), rows that begin on a cache line (a multiple of 8) and that do not, ragged last tiles, an odd number of
 # stages.
 LARGE = [(25, 6000, 1500), (30, 9000, 600), (700, 900, 1088), (600, 1500, 1100), (1100, 1300, 640), (1537, 4100, 320), (2049, 4100, 200), (1300, 6200, 1000),
@@ -202,7 +202,7 @@ def test_large_linear_of_strided_rows(m, n, k, pad):
 
 @pytest.mark.parametrize("kind", ["linear", "gemm"])
 def test_large_products_repeat_and_leave_nan_in_its_row(kind):
-    """Both tiled kernels: the same bits on every run; a NaN block reaches its own weight row, and with 4-bit x its own x row, and nothing else."""
+    """Tiled kernels: the same bits on every run; a NaN block reaches its own weight row, and with 4-bit x its own x row, and nothing else."""
     for m, n, k in ((1100, 1300, 640), (2100, 4000, 416)):
         args, _, _ = case(kind, m, n, k, False, False, False, torch.float32, make=make_fast)
         first = product(kind, **args)
@@ -341,6 +341,38 @@ def test_products_on_two_streams_and_in_a_graph():
         eager = chain(new, bufs())
         torch.cuda.synchronize()
         assert torch.equal(gb[3], eager)
+
+
+@pytest.mark.parametrize("kind", ["linear", "gemm"])
+@pytest.mark.parametrize("m,n,k,gated", [(1, 512, 1024, False), (18, 8049, 1280, False), (64, 16384, 1024, False), (130, 9000, 1111, False), (250, 8200, 1000, True),
+                                         (384, 16384, 512, False), (2048, 8192, 300, True)])
+def test_every_tile_repeats_and_replays(kind, m, n, k, gated):
+    """A captured call without one before it, replayed between eager ones: the same bits every time, and a NaN block of the weights reaches its own column
+    alone."""
+    args, want, size = case(kind, m, n, k, gated, False, False, torch.float32, make=make_fast)
+    x, w, w2 = args["x"], args["w"], args["w2"] or (None, None)
+    out = torch.zeros(m, n, device="cuda")
+    act = (ptr(x), x.stride(0)) if kind == "linear" else (ptr(x[0]), ptr(x[1]))
+    fn = N.lib().mv_op_linear_mxfp4 if kind == "linear" else N.lib().mv_op_gemm_mxfp4
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        N.check(fn(stream(), m, n, k, *act, ptr(w[0]), ptr(w[1]), ptr(w2[0]), ptr(w2[1]), None, None, None, 1, ptr(out)))
+    graph.replay()
+    torch.cuda.synchronize()
+    within(out, want, size, k, torch.float32)
+    first = out.clone()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        eager = product(kind, **args)
+        torch.cuda.synchronize()
+        assert torch.equal(out, first) and torch.equal(eager, first)
+    w[1][n // 2, -1] = 255
+    graph.replay()
+    torch.cuda.synchronize()
+    nan = torch.isnan(out)
+    assert bool(nan[:, n // 2].all()) and int(nan.sum()) == m and torch.equal(out[~nan], first[~nan])
 
 
 @pytest.mark.parametrize("kind", ["linear", "gemm"])
