@@ -182,7 +182,8 @@ typedef struct mv_logit_controls {
     int32_t pad0;
 } mv_logit_controls;
 /* logits (and uncond) [rows][ld], dtype MV_BF16 or MV_F32 -> out [rows][ld_out] of out_dtype; per token, in fp32, rounded once:
- *   with uncond: x = g x + (1 - g) u (an x of -inf stays);  repetition, then - (n frequency + presence);  + bias;  mask bit 0: -inf, NaN or not.
+ *   with uncond: x = g x + (1 - g) u;  repetition, then - (n frequency + presence);  + bias;  mask bit 0: -inf, NaN or not.
+ * The mix leaves x as it is where x is infinite, where g = 1, and where u is -inf with g > 1; only its result has to lie in the range of fp32, not its terms.
  * An engine's [2u] conditioned, [2u + 1] unconditioned rows are logits, uncond = logits + vocab, ld = 2 vocab.  `out` may be `logits` (same dtype
  * and stride).  allowed (optional) [rows]: tokens the mask leaves, 0 when a grammar has run into a dead end (the row is -inf throughout).
  * Enqueued on `stream`: no allocation, no scratch memory, no synchronisation.  out feeds mv_op_sample with a row of zeros as the unconditioned

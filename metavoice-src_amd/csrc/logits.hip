@@ -1,7 +1,7 @@
 // Controls on next-token logits, before the sampler: guidance mix, penalties for repeated tokens, biases, grammar masks.
 //
 // For token v of a row, in fp32, rounded once at the end:
-//   x = logits[v]                                     with `uncond`: -inf stays, else g * logits[v] + (1 - g) * uncond[v]
+//   x = logits[v]                                     with `uncond`: g * logits[v] + (1 - g) * uncond[v], see lc_mix
 //   v occurs in the history:                          x = x > 0 ? x / repetition : x * repetition
 //   v occurs n > 0 times behind the prompt:           x = x - (n * frequency + presence)
 //   v is in the bias list (its last entry holds):     x = x + bias
@@ -66,6 +66,16 @@ __device__ __forceinline__ f32x4_t lc_load(const void* base, int64_t at, int lef
             if (i < left) r[i] = bf2f(p[i]);
     }
     return r;
+}
+
+// Guidance mix.  An infinite logit stays, guidance 1 is the conditioned row whatever lies beside it, and beyond 1 a token that the unconditioned row alone
+// excludes (u = -inf) stays too, where the formula would make it the only token.  The terms may leave the range of fp32 where the mix does not (both rows
+// masked by the type's lowest value): such a mix is taken in 64 bits.
+__device__ __forceinline__ float lc_mix(float g, float x, float u) {
+    const float y = g * x + (1.f - g) * u;
+    if (fabsf(y) < INFINITY) return y;
+    if (fabsf(x) == INFINITY || g == 1.f || (u == -INFINITY && g > 1.f)) return x;
+    return (float)((double)g * x + (1.0 - (double)g) * u);
 }
 
 #define LC_AHEAD 4  // history ids per thread that are asked for at once
@@ -161,8 +171,7 @@ __global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const Contro
         if (left <= 0) break;
         if (a.uncond) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (x[j][i] != -INFINITY) x[j][i] = g * x[j][i] + (1.f - g) * u[j][i];
+            for (int i = 0; i < 4; ++i) x[j][i] = lc_mix(g, x[j][i], u[j][i]);
         }
         if (counted) {
             const u32x4 n4 = *(const u32x4*)&count[k];

@@ -16,7 +16,8 @@ def controls(logits, uncond=None, guidance=None, repetition=None, presence=None,
             x, s = out[r], size[r]
             if uncond is not None:
                 g = float(guidance[r])
-                live = x != -np.inf
+                # an infinite logit, a guidance of 1, and beyond 1 a token that the unconditioned row excludes: x stays
+                live = ~(np.isinf(x) | (g == 1) | ((uncond[r] == -np.inf) & (g > 1)))
                 s[live] = np.abs(g * x[live]) + np.abs((1 - g) * uncond[r][live])
                 x[live] = g * x[live] + (1 - g) * uncond[r][live]
             if history is not None:
