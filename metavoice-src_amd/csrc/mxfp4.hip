@@ -125,12 +125,18 @@ struct MxArgs {
     int32_t x_direct, s_direct;  // rows of x and of scales are aligned to 4 bytes
 };
 
+// silu(v) = v / (1 + exp(-v)).  The fast exponential rounds its argument times log2(e), an error of up to |v| 2^-24 of the result: nothing beside half a step
+// of bf16 (2^-8), but tens of steps of fp32.  So fp32 outputs take the accurate one (256 x 5632 x 2048 in codes 10.6 -> 11.4 us; bf16 outputs would lose 3 - 6 %
+// to it, and as much to a choice per element: the choice stands around whole runs of columns).
+__device__ __forceinline__ float mx_silu_bf16(float v) { return v / (1.0f + __expf(-v)); }
+__device__ __forceinline__ float mx_silu_f32(float v) { return v / (1.0f + expf(-v)); }
+
 // y = x . w + bias (gated: silu(y) * (x . w2 + bias2)) + residual, in fp32, rounded once
 __device__ __forceinline__ void mx_store(const MxArgs& a, int m, int n, float v, float v2) {
     if (a.bias) v += bf2f(a.bias[n]);
     if (a.w2) {
         if (a.bias2) v2 += bf2f(a.bias2[n]);
-        v = v / (1.0f + __expf(-v)) * v2;
+        v = (a.out_f32 ? mx_silu_f32(v) : mx_silu_bf16(v)) * v2;
     }
     const int64_t at = (int64_t)m * a.N + n;
     if (a.out_f32) {
@@ -161,11 +167,17 @@ __device__ __forceinline__ void mx_store8(const MxArgs& a, int m, int n, float (
 #pragma unroll
             for (int e = 0; e < 8; ++e) v2[e] += e & 1 ? bf_hi(b[e >> 1]) : bf_lo(b[e >> 1]);
         }
+        if (!a.out_f32) {  // fp32: below
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.0f + __expf(-v[e])) * v2[e];
+            for (int e = 0; e < 8; ++e) v[e] = mx_silu_bf16(v[e]) * v2[e];
+        }
     }
     const int64_t at = (int64_t)m * a.N + n;
     if (a.out_f32) {
+        if (a.w2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = mx_silu_f32(v[e]) * v2[e];
+        }
         if (a.res) {
             const f32x4_any lo = *(const f32x4_any*)((const float*)a.res + at), hi = *(const f32x4_any*)((const float*)a.res + at + 4);
 #pragma unroll
