@@ -139,7 +139,8 @@ int mv_op_attention_rows(void* stream, int32_t batch, int32_t T, int32_t n_head,
  * 0 0.5 1 1.5 2 3 4 6) times 2^(s - 127), s its scale byte; s = 255: NaN.
  *   codes  [rows][16 nb] bytes (column 2j low, 2j + 1 high nibble of byte j; zero past K), 16-byte aligned;   scales [rows][nb] bytes
  * A call with no row or no column (M, N or rows 0) does nothing.  Sizes and strides count elements; strides need no alignment, but rows that
- * begin on 128 bytes (K a multiple of 256) are read fastest.  Outputs lie apart from inputs except where a call says otherwise.
+ * begin on 128 bytes (K a multiple of 256) are read fastest.  Outputs lie apart from inputs and from each other except where a call says
+ * otherwise; calls where they share a byte are refused.
  *
  * mv_op_quantize_mxfp4: w [N][ldw], dtype MV_BF16 or MV_F32 -> codes, scales and, when not NULL, the values they stand for as bf16 [N][K]
  * (`dequantised` may be w itself when w is bf16 and ldw = K).  Block exponent floor(log2 max|w|) - 2, at least -127; codes rounded to nearest,
@@ -183,9 +184,12 @@ typedef struct mv_logit_controls {
 } mv_logit_controls;
 /* logits (and uncond) [rows][ld], dtype MV_BF16 or MV_F32 -> out [rows][ld_out] of out_dtype; per token, in fp32, rounded once:
  *   with uncond: x = g x + (1 - g) u;  repetition, then - (n frequency + presence);  + bias;  mask bit 0: -inf, NaN or not.
- * The mix leaves x as it is where x is infinite, where g = 1, and where u is -inf with g > 1; only its result has to lie in the range of fp32, not its terms.
- * An engine's [2u] conditioned, [2u + 1] unconditioned rows are logits, uncond = logits + vocab, ld = 2 vocab.  `out` may be `logits` (same dtype
- * and stride).  allowed (optional) [rows]: tokens the mask leaves, 0 when a grammar has run into a dead end (the row is -inf throughout).
+ * The mix leaves x as it is where x is infinite, where g = 1, and where u is -inf with g > 1; only its result, not its terms, has to lie in the
+ * range of fp32.
+ * An engine's [2u] conditioned, [2u + 1] unconditioned rows are logits, uncond = logits + vocab, ld = 2 vocab.  `out` may be `logits` or `uncond`
+ * (same dtype and stride); else outputs lie apart from inputs and from each other (calls where they share a byte are refused, but for interleaved
+ * rows of two different strides).  allowed (optional) [rows]: tokens the mask leaves, 0 when a grammar has run into a dead end (the row is -inf
+ * throughout).
  * Enqueued on `stream`: no allocation, no scratch memory, no synchronisation.  out feeds mv_op_sample with a row of zeros as the unconditioned
  * logits, guidance_scale 1, one_minus_guidance 0. */
 int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, int32_t dtype, const void* logits, const void* uncond, int64_t ld,

@@ -243,6 +243,18 @@ extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, i
     a.chunks = (uint32_t)((vocab + (int64_t)LC_CHUNK - 1) / LC_CHUNK);
     a.groups = a.chunks + (allowed ? 1 : 0);
     if ((int64_t)a.groups * rows > 0x7FFFFFFF) return mv_fail(MV_ERR_INVALID, "logit_controls: rows=%d vocab=%d is too large", rows, vocab);
+    const int64_t words = (vocab + 31LL) / 32;
+    const auto row_of = [&](const void* p, int64_t stride, size_t e) { return OpRows{p, rows, std::min(stride, OP_FAR) * (int64_t)e, (int64_t)vocab * (int64_t)e}; };
+    const auto per_row = [&](const void* p) { return op_bytes(p, rows, 4); };
+    const OpRows y = row_of(out, ld_out, eout), n = per_row(allowed), history{c.history, rows, std::min(c.ld_history, OP_FAR) * 4, c.history_cap * 4LL};
+    const OpRows ids{c.bias_ids, c.ld_bias ? rows : 1, std::min(c.ld_bias, OP_FAR) * 4, c.n_bias * 4LL}, bias{c.bias, ids.rows, ids.stride, ids.width};
+    if (op_overlap(y, n) || (out != logits && op_overlap(y, row_of(logits, ld, ein))) || (out != uncond && op_overlap(y, row_of(uncond, ld, ein))))
+        return mv_fail(MV_ERR_INVALID, "logit_controls: out on top of a part of its inputs or of allowed");
+    for (const OpRows& b : {row_of(logits, ld, ein), row_of(uncond, ld, ein), per_row(c.guidance), per_row(c.repetition), per_row(c.presence), per_row(c.frequency),
+                            per_row(c.history_len), per_row(c.prompt_len), per_row(c.mask_index), history, ids, bias, OpRows{c.masks, c.n_masks, std::min(c.ld_mask, OP_FAR) * 4, words * 4}}) {
+        if (op_overlap(n, b)) return mv_fail(MV_ERR_INVALID, "logit_controls: allowed on top of an input");
+        if (b.p != logits && b.p != uncond && op_overlap(y, b)) return mv_fail(MV_ERR_INVALID, "logit_controls: out on top of an input");
+    }
     OpDevice dev((hipStream_t)stream, out);
     LC_TRY(dev.status());
     const dim3 grid = op_grid((uint64_t)a.groups * rows), block(LC_THREADS);

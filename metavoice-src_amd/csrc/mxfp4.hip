@@ -909,19 +909,24 @@ hipError_t launch_products(hipStream_t s, MxArgs a, bool x4) {
 }
 
 // the checks that both products share; null: fine
-const char* product_fault(int32_t M, int32_t N, int32_t K, const void* x, const void* codes, const void* scales, const void* codes2, const void* scales2, const void* bias,
-                          const void* bias2, const void* residual, int32_t out_dtype, const void* out) {
+const char* product_fault(int32_t M, int32_t N, int32_t K, const OpRows& x, const void* x_scales, const void* codes, const void* scales, const void* codes2, const void* scales2,
+                          const void* bias, const void* bias2, const void* residual, int32_t out_dtype, const void* out) {
     if (M < 0 || N < 0 || K < 1) return "M and N must not be negative, K must be positive";
     if (std::max({M, N, K}) > 0x7FFFFFFF - 4096) return "M, N or K is too large";
     if (out_dtype != MV_BF16 && out_dtype != MV_F32) return "out_dtype must be MV_BF16 or MV_F32";
     if (M == 0 || N == 0) return nullptr;
     if (!codes || !scales || !out) return "null argument";
-    if (out == x) return "out on top of x";
     if (!codes2 != !scales2) return "codes2 and scales2 go together";
     if (bias2 && !codes2) return "bias2 without codes2";
     if (!op_aligned(codes, 16) || !op_aligned(codes2, 16)) return "codes must be aligned to 16 bytes";
     const size_t esz = out_dtype == MV_F32 ? 4 : 2;
     if (!op_aligned(out, esz) || !op_aligned(residual, esz) || !op_aligned(bias, 2) || !op_aligned(bias2, 2)) return "a buffer is not aligned to its element";
+    const int64_t nb = ((int64_t)K + 31) / 32;
+    const OpRows y = op_bytes(out, M, (int64_t)N * (int64_t)esz);
+    if (residual != out && op_overlap(y, op_bytes(residual, M, (int64_t)N * (int64_t)esz))) return "out on top of a part of the residual";
+    for (const OpRows& b : {x, op_bytes(x_scales, M, nb), op_bytes(codes, N, 16 * nb), op_bytes(codes2, N, 16 * nb), op_bytes(scales, N, nb), op_bytes(scales2, N, nb),
+                            op_bytes(bias, N, 2), op_bytes(bias2, N, 2)})
+        if (op_overlap(y, b)) return "out on top of an input";
     return nullptr;
 }
 
@@ -938,8 +943,12 @@ int mv_op_quantize_mxfp4(void* stream, int32_t N, int32_t K, int32_t dtype, cons
     const size_t esz = dtype == MV_F32 ? 4 : 2;
     if (!op_aligned(w, esz) || !op_aligned(codes, 16) || !op_aligned(dequantised, 2))
         return mv_fail(MV_ERR_INVALID, "quantize_mxfp4: codes must be aligned to 16 bytes, the other buffers to their element");
-    if (codes == w || scales == w || (dequantised == w && (dtype != MV_BF16 || ldw != K)))
-        return mv_fail(MV_ERR_INVALID, "quantize_mxfp4: an output on top of w (dequantised may be, with bf16 and ldw = K)");
+    const int64_t nb = ((int64_t)K + 31) / 32;
+    const OpRows in{w, N, std::min(ldw, OP_FAR) * (int64_t)esz, K * (int64_t)esz}, c = op_bytes(codes, N, 16 * nb), s = op_bytes(scales, N, nb), d = op_bytes(dequantised, N, (int64_t)K * 2);
+    const bool in_place = dequantised == w && dtype == MV_BF16 && ldw == K;
+    if (op_overlap(c, in) || op_overlap(s, in) || (!in_place && op_overlap(d, in)))
+        return mv_fail(MV_ERR_INVALID, "quantize_mxfp4: an output on top of w (dequantised may be w, with bf16 and ldw = K)");
+    if (op_overlap(c, s) || op_overlap(c, d) || op_overlap(s, d)) return mv_fail(MV_ERR_INVALID, "quantize_mxfp4: an output on top of another");
     OpDevice dev((hipStream_t)stream, codes);
     MX_TRY(dev.status());
     QuantArgs a;
@@ -967,9 +976,9 @@ int mv_op_quantize_mxfp4(void* stream, int32_t N, int32_t K, int32_t dtype, cons
 
 int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x, int64_t ldx, const void* codes, const void* scales, const void* codes2,
                        const void* scales2, const void* bias, const void* bias2, const void* residual, int32_t out_dtype, void* out) {
-    const char* fault = product_fault(M, N, K, x, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out);
-    if (!fault && ldx < K) fault = "ldx below K";
+    const char* fault = ldx < K ? "ldx below K" : nullptr;
     if (!fault && M > 0 && N > 0 && (!x || !op_aligned(x, 2))) fault = "x is null or not aligned to its element";
+    if (!fault) fault = product_fault(M, N, K, OpRows{x, M, std::min(ldx, OP_FAR) * 2, (int64_t)K * 2}, nullptr, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out);
     if (fault) return mv_fail(MV_ERR_INVALID, "linear_mxfp4: %s (M=%d N=%d K=%d)", fault, M, N, K);
     if (M == 0 || N == 0) return MV_OK;
     OpDevice dev((hipStream_t)stream, out);
@@ -982,8 +991,8 @@ int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void
 
 int mv_op_gemm_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x_codes, const void* x_scales, const void* codes, const void* scales,
                      const void* codes2, const void* scales2, const void* bias, const void* bias2, const void* residual, int32_t out_dtype, void* out) {
-    const char* fault = product_fault(M, N, K, x_codes, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out);
-    if (!fault && M > 0 && N > 0 && (!x_codes || !x_scales || !op_aligned(x_codes, 16))) fault = "x_codes must be aligned to 16 bytes, x_scales not null";
+    const char* fault = M > 0 && N > 0 && (!x_codes || !x_scales || !op_aligned(x_codes, 16)) ? "x_codes must be aligned to 16 bytes, x_scales not null" : nullptr;
+    if (!fault) fault = product_fault(M, N, K, op_bytes(x_codes, M, ((int64_t)K + 31) / 32 * 16), x_scales, codes, scales, codes2, scales2, bias, bias2, residual, out_dtype, out);
     if (fault) return mv_fail(MV_ERR_INVALID, "gemm_mxfp4: %s (M=%d N=%d K=%d)", fault, M, N, K);
     if (M == 0 || N == 0) return MV_OK;
     OpDevice dev((hipStream_t)stream, out);

@@ -3,7 +3,7 @@ with the tolerance of test_logits_gpu.py."""
 import pytest
 import torch
 
-from test_logits_gpu import BF, F, check, hip
+from test_logits_gpu import BF, CODE, F, N, check, hip, ptr, stream, struct
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,21 @@ def test_tokens_that_one_row_excludes():
     u = torch.tensor([[1.0, 1.0, -INF, -INF]] * 3)
     out, _ = hip(x.cuda(), u.cuda(), dict(guidance=torch.tensor([0.5, 1.0, 3.0]).cuda()), F)
     assert out.tolist() == [[1.5, -INF, -INF, -INF], [2.0, -INF, 2.0, -INF], [4.0, -INF, 2.0, -INF]]
+
+
+@pytest.mark.parametrize("dt", [BF, F])
+def test_outputs_beside_their_inputs(dt):
+    """Rows of outputs may lie between rows of inputs, and on top of either row of a pair."""
+    g = torch.Generator().manual_seed(4)
+    rows, v = 5, 333
+    data = torch.randn(rows, 4, v, generator=g).to(dt)
+    d = dict(guidance=torch.full((rows,), 1.5).cuda())
+    want = hip(data[:, 0].contiguous().cuda(), data[:, 1].contiguous().cuda(), d, dt)[0]
+    for place in range(4):
+        room = data.cuda()
+        c = struct(d)
+        N.check(N.lib().mv_op_logit_controls(stream(), rows, v, CODE[dt], ptr(room), ptr(room[:, 1]), 4 * v, c, CODE[dt], ptr(room[:, place]), 4 * v, None))
+        torch.cuda.synchronize()
+        assert torch.equal(room[:, place], want)
+        rest = [i for i in range(4) if i != place]
+        assert torch.equal(room[:, rest].cpu(), data[:, rest])

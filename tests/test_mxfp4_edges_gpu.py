@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import mxfp4 as o_mx
-from test_mxfp4_gpu import check_quantised, dev, hip_quantize, product
+from test_mxfp4_gpu import N, check_quantised, dev, hip_quantize, product, ptr, stream
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,19 @@ def test_quantiser_of_the_smallest_fp32_numbers():
     w = torch.cat([bits.view(torch.float32), row, (bits >> 1).view(torch.float32)])
     w = torch.cat([w, -w]).cuda()
     check_quantised(w, *hip_quantize(w))
+
+
+def test_an_output_in_a_gap_of_x():
+    """A whole output between two rows of strided x, and the rows themselves stay."""
+    m, n, k, ld = 3, 40, 96, 1000
+    g = torch.Generator().manual_seed(2)
+    room = torch.randn(m, ld, generator=g).bfloat16().cuda()
+    keep = room.clone()
+    w = tuple(map(dev, o_mx.quantize(torch.randn(n, k, generator=g).double().numpy())))
+    want = product("linear", room[:, :k], w, k=k)
+    for row, at in ((0, k), (1, 500), (2, ld - m * n)):
+        room.copy_(keep)
+        out = room.view(-1)[row * ld + at:row * ld + at + m * n]
+        N.check(N.lib().mv_op_linear_mxfp4(stream(), m, n, k, ptr(room), ld, ptr(w[0]), ptr(w[1]), None, None, None, None, None, 0, ptr(out)))
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(m, n), want) and torch.equal(room[:, :k], keep[:, :k])
