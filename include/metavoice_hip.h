@@ -158,6 +158,12 @@ int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void
 int mv_op_gemm_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x_codes, const void* x_scales, const void* codes,
                      const void* scales, const void* codes2, const void* scales2, const void* bias, const void* bias2, const void* residual,
                      int32_t out_dtype, void* out);
+/* The kernel that a product of these sizes takes: nothing is launched and no GPU is needed, the addresses (one of scales for all operands) count by
+ * their alignment alone.  out[0] kernel (0-2: few rows; 3-7: tiles of 64 x 64, 64 x 128, 128 x 128, 128 x 256, 256 x 256), [1] rows on whole lines,
+ * [2] x and [3] scales by direct transfers, [4] steps of a wave or stages of a tile, [5] stages in LDS (tiles), [6] whole groups of 16 scales,
+ * [7] groups asked for ahead (tiles).  For tests that mean to reach a kernel. */
+int mv_debug_mxfp4_kernel(int32_t x4, int32_t M, int32_t N, int32_t K, int64_t ldx, int32_t gated, uint64_t x, uint64_t codes, uint64_t scales,
+                          int32_t* out);
 
 /* Controls on next-token logits before the sampler (no reference equivalent).  The struct lies on the host, its pointers are DEVICE buffers;
  * NULL switches a control off. */

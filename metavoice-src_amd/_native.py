@@ -103,6 +103,7 @@ SYMBOLS = [
     ("mv_op_quantize_mxfp4", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P]),
     ("mv_op_linear_mxfp4", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P, _P, _P, _P, _P, _P, C.c_int32, _P]),
     ("mv_op_gemm_mxfp4", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int32, _P]),
+    ("mv_debug_mxfp4_kernel", C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint64, C.POINTER(C.c_int32)]),
     ("mv_op_logit_controls", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int64, C.POINTER(mv_logit_controls), C.c_int32, _P, C.c_int64, _P]),
     ("mv_stage2_create", C.c_int, [C.POINTER(mv_stage2_config), C.POINTER(_P)]),
     ("mv_stage2_destroy", C.c_int, [_P]),

@@ -832,8 +832,8 @@ hipError_t allow_lds(int bytes) {
     return e;
 }
 
-template <bool X4, int KS, int WN, int WM, int TW, int TX, bool GATED>
-hipError_t launch_tiles(hipStream_t s, MxArgs a) {
+template <bool GATED, bool X4, int KS, int WN, int WM, int TW, int TX>
+hipError_t launch_tiles(hipStream_t s, MxArgs a, Tile<X4, KS, WN, WM, TW, TX>) {
     typedef Tile<X4, KS, WN, WM, TW, TX> T;
     constexpr int NOUT = GATED ? T::BN / 2 : T::BN;
     const uint32_t tiles_m = (uint32_t)((a.M + T::BM - 1) / T::BM);
@@ -876,36 +876,72 @@ double tiles_us(const MxArgs& a, const TileCost& c) {
     return c.call + rounds * (c.round + a.nb * (a.s_direct ? 1.0 : 1.4) * (c.block + c.full * std::min(1.0, tiles / 256)));
 }
 
-template <bool X4, bool GATED, bool LINES>
-hipError_t choose(hipStream_t s, const MxArgs& a) {
-    // Tiles of the first kernel in 16s of rows and columns.  With bf16 rows more columns come before more rows, since a row costs what 4 columns do.
-    constexpr int M3 = X4 ? 2 : 1, N3 = X4 ? 2 : 4;
-    const double r1 = rows_us<X4>(a, 1, 1), r2 = rows_us<X4>(a, 1, 2), r3 = rows_us<X4>(a, M3, N3), rows = std::min({r1, r2, r3});
+// The kernels: three of the first kind (in 16s of rows and columns 1 x 1, 1 x 2, and 1 x 4 or, with codes, 2 x 2: with bf16 rows more columns come before more
+// rows, since a row costs what 4 columns do), then five of the second.
+constexpr int MX_ROW_TILES = 3;
+constexpr int MX_TALL[2][2] = {{1, 4}, {2, 2}};
+template <bool X4, class F>
+auto with_tile(int tile, const F& f) {
+    switch (tile) {
+        case 0: return f(Tile<X4, X4 ? 2 : 4, X4 ? 2 : 1, 2, X4 ? 1 : 2, 1>());
+        case 1: return f(Tile<X4, 2, 2, 2, 2, 1>());
+        case 2: return f(Tile<X4, 2, 2, 2, 2, 2>());
+        case 3: return f(Tile<X4, 1, 4, 2, 2, 2>());
+        default: return f(Tile<X4, 1, 2, 4, 4, 2>());
+    }
+}
+
+// the fastest by the estimate: 0 .. 2 of the first kind, 3 .. 7 of the second
+template <bool X4>
+int choose(const MxArgs& a) {
+    const double r1 = rows_us<X4>(a, 1, 1), r2 = rows_us<X4>(a, 1, 2), r3 = rows_us<X4>(a, MX_TALL[X4][0], MX_TALL[X4][1]), rows = std::min({r1, r2, r3});
     const int64_t x_row = X4 ? (int64_t)a.nb * 16 : a.ldx * 2;
     // the second kernel counts bytes within a workgroup's rows in 32 bits, and its threads are one dimension of a grid
-    if (x_row <= 1 << 23 && a.nb <= 1 << 19 && ((a.M + 63ll) / 64) * ((a.N * (GATED ? 2ll : 1ll) + 63) / 64) < 1 << OP_GRID_BITS) {
+    if (x_row <= 1 << 23 && a.nb <= 1 << 19 && ((a.M + 63ll) / 64) * ((a.N * (a.w2 ? 2ll : 1ll) + 63) / 64) < 1 << OP_GRID_BITS) {
         const TileCost* c = MX_COST[X4];
-        const double t1 = tiles_us(a, c[0]), t2 = tiles_us(a, c[1]), t3 = tiles_us(a, c[2]);
-        const double t4 = a.x_direct ? tiles_us(a, c[3]) : 1e30, t5 = a.x_direct ? tiles_us(a, c[4]) : 1e30, tiles = std::min({t1, t2, t3, t4, t5});
-        if (tiles < rows) {
-            if (t1 == tiles) return launch_tiles<X4, X4 ? 2 : 4, X4 ? 2 : 1, 2, X4 ? 1 : 2, 1, GATED>(s, a);
-            if (t2 == tiles) return launch_tiles<X4, 2, 2, 2, 2, 1, GATED>(s, a);
-            if (t3 == tiles) return launch_tiles<X4, 2, 2, 2, 2, 2, GATED>(s, a);
-            if (t4 == tiles) return launch_tiles<X4, 1, 4, 2, 2, 2, GATED>(s, a);
-            return launch_tiles<X4, 1, 2, 4, 4, 2, GATED>(s, a);
-        }
+        double t[5];
+        for (int i = 0; i < 5; ++i) t[i] = i < 3 || a.x_direct ? tiles_us(a, c[i]) : 1e30;
+        const double tiles = *std::min_element(t, t + 5);
+        if (tiles < rows) return MX_ROW_TILES + (int)(std::find(t, t + 5, tiles) - t);
     }
-    if (r1 == rows) return launch_rows<X4, GATED, LINES, 1, 1>(s, a);
-    if (r2 == rows) return launch_rows<X4, GATED, LINES, 1, 2>(s, a);
-    return launch_rows<X4, GATED, LINES, M3, N3>(s, a);
+    return r1 == rows ? 0 : r2 == rows ? 1 : 2;
+}
+
+// what decides among the forms of a kernel, by addresses and strides; true: whole lines
+bool product_form(MxArgs& a, bool x4) {
+    a.x_direct = x4 || (op_aligned(a.x, 4) && a.ldx % 2 == 0);
+    a.s_direct = a.nb % 4 == 0 && op_aligned(a.ws, 4) && op_aligned(a.ws2, 4) && op_aligned(a.xs, 4);
+    return a.nb % 8 == 0 && op_aligned(a.w, 128) && op_aligned(a.w2, 128) && op_aligned(a.x, 128) && (x4 || a.ldx % 64 == 0);
+}
+
+template <bool X4, bool GATED, bool LINES>
+hipError_t launch(hipStream_t s, const MxArgs& a) {
+    const int kernel = choose<X4>(a);
+    if (kernel == 0) return launch_rows<X4, GATED, LINES, 1, 1>(s, a);
+    if (kernel == 1) return launch_rows<X4, GATED, LINES, 1, 2>(s, a);
+    if (kernel == 2) return launch_rows<X4, GATED, LINES, MX_TALL[X4][0], MX_TALL[X4][1]>(s, a);
+    return with_tile<X4>(kernel - MX_ROW_TILES, [&](auto tile) { return launch_tiles<GATED>(s, a, tile); });
 }
 
 hipError_t launch_products(hipStream_t s, MxArgs a, bool x4) {
-    a.x_direct = x4 || (op_aligned(a.x, 4) && a.ldx % 2 == 0);
-    a.s_direct = a.nb % 4 == 0 && op_aligned(a.ws, 4) && op_aligned(a.ws2, 4) && op_aligned(a.xs, 4);
-    const bool lines = a.nb % 8 == 0 && op_aligned(a.w, 128) && op_aligned(a.w2, 128) && op_aligned(a.x, 128) && (x4 || a.ldx % 64 == 0);
-    if (lines) return x4 ? (a.w2 ? choose<true, true, true>(s, a) : choose<true, false, true>(s, a)) : (a.w2 ? choose<false, true, true>(s, a) : choose<false, false, true>(s, a));
-    return x4 ? (a.w2 ? choose<true, true, false>(s, a) : choose<true, false, false>(s, a)) : (a.w2 ? choose<false, true, false>(s, a) : choose<false, false, false>(s, a));
+    if (product_form(a, x4)) return x4 ? (a.w2 ? launch<true, true, true>(s, a) : launch<true, false, true>(s, a)) : (a.w2 ? launch<false, true, true>(s, a) : launch<false, false, true>(s, a));
+    return x4 ? (a.w2 ? launch<true, true, false>(s, a) : launch<true, false, false>(s, a)) : (a.w2 ? launch<false, true, false>(s, a) : launch<false, false, false>(s, a));
+}
+
+template <bool X4>
+void describe(const MxArgs& a, bool lines, int32_t* out) {
+    const int kernel = choose<X4>(a), tile = kernel - MX_ROW_TILES;
+    out[0] = kernel;
+    out[1] = lines;
+    out[2] = a.x_direct;
+    out[3] = a.s_direct;
+    out[4] = tile < 0 ? (a.nb + MX_WAVES * (lines ? 8 : 4) - 1) / (MX_WAVES * (lines ? 8 : 4)) : with_tile<X4>(tile, [&](auto t) {
+        const int blocks = 16 / decltype(t)::GROUP;
+        return (a.nb + blocks - 1) / blocks;
+    });
+    out[5] = tile < 0 ? 0 : with_tile<X4>(tile, [](auto t) { return (int)decltype(t)::NBUF; });
+    out[6] = a.nb / 16;
+    out[7] = tile < 0 ? 0 : with_tile<X4>(tile, [](auto t) { return (int)decltype(t)::AHEAD; });
 }
 
 // the checks that both products share; null: fine
@@ -1000,6 +1036,15 @@ int mv_op_gemm_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* 
     MxArgs a{x_codes, (const unsigned char*)x_scales, (const unsigned char*)codes, (const unsigned char*)scales, (const unsigned char*)codes2,
              (const unsigned char*)scales2, (const bf16_t*)bias, (const bf16_t*)bias2, residual, out, 0, M, N, K, (K + 31) / 32, out_dtype == MV_F32, 0, 0, 0};
     MX_TRY(launch_products((hipStream_t)stream, a, true));
+    return MV_OK;
+}
+
+int mv_debug_mxfp4_kernel(int32_t x4, int32_t M, int32_t N, int32_t K, int64_t ldx, int32_t gated, uint64_t x, uint64_t codes, uint64_t scales, int32_t* out) {
+    if (M < 1 || N < 1 || K < 1 || std::max({M, N, K}) > 0x7FFFFFFF - 4096 || (!x4 && ldx < K) || !out) return mv_fail(MV_ERR_INVALID, "debug_mxfp4_kernel: bad argument");
+    const unsigned char *w = (const unsigned char*)codes, *ws = (const unsigned char*)scales;
+    MxArgs a{(const void*)x, x4 ? ws : nullptr, w, ws, gated ? w : nullptr, gated ? ws : nullptr, nullptr, nullptr, nullptr, nullptr, x4 ? 0 : ldx, M, N, K, (K + 31) / 32, 0, 0, 0, 0};
+    const bool lines = product_form(a, x4 != 0);
+    x4 ? describe<true>(a, lines, out) : describe<false>(a, lines, out);
     return MV_OK;
 }
 
