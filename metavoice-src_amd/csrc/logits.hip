@@ -17,6 +17,7 @@
 #include "op_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #define LC_THREADS 512
 #define LC_GROUPS 2                                // groups of 4 consecutive tokens per thread
@@ -70,17 +71,17 @@ __device__ __forceinline__ f32x4_t lc_load(const void* base, int64_t at, int lef
 
 // Guidance mix.  An infinite logit stays, guidance 1 is the conditioned row whatever lies beside it, and beyond 1 a token that the unconditioned row alone
 // excludes (u = -inf) stays too, where the formula would make it the only token.  The terms may leave the range of fp32 where the mix does not (both rows
-// masked by the type's lowest value): such a mix is taken in 64 bits.
+// masked by the type's lowest value): then the difference of the rows is taken first, in halves, none of which is larger than the mix or the rows.
 __device__ __forceinline__ float lc_mix(float g, float x, float u) {
     const float y = g * x + (1.f - g) * u;
     if (fabsf(y) < INFINITY) return y;
     if (fabsf(x) == INFINITY || g == 1.f || (u == -INFINITY && g > 1.f)) return x;
-    return (float)((double)g * x + (1.0 - (double)g) * u);
+    return 2.f * (0.5f * x + (g - 1.f) * (0.5f * x - 0.5f * u));
 }
 
 #define LC_AHEAD 4  // history ids per thread that are asked for at once
 
-template <bool IN32, bool OUT32>
+template <bool IN32, bool OUT32, bool GUIDED>
 __global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const ControlArgs a) {
     __shared__ __attribute__((aligned(16))) uint32_t count[LC_CHUNK];  // bit 31: in the prompt; below: occurrences behind it
     __shared__ __attribute__((aligned(16))) uint32_t entry[LC_CHUNK];  // 1 + the bias entry that holds, 0: none
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const Contro
     for (int j = 0; j < LC_GROUPS; ++j) {
         const int v = v0 + (j * LC_THREADS + tid) * 4, left = a.vocab - v;
         x[j] = left > 0 ? lc_load<IN32>(a.logits, (int64_t)row * a.ld + v, left) : f32x4_t{0, 0, 0, 0};
-        u[j] = left > 0 && a.uncond ? lc_load<IN32>(a.uncond, (int64_t)row * a.ld + v, left) : f32x4_t{0, 0, 0, 0};
+        u[j] = GUIDED && left > 0 ? lc_load<IN32>(a.uncond, (int64_t)row * a.ld + v, left) : f32x4_t{0, 0, 0, 0};
         word[j] = left > 0 && mask ? mask[v >> 5] : 0xFFFFFFFFu;
     }
     int seen[LC_AHEAD], extra = -1;
@@ -163,13 +164,13 @@ __global__ void __launch_bounds__(LC_THREADS) logit_controls_kernel(const Contro
         __syncthreads();
     }
 
-    const float g = a.uncond ? c.guidance[row] : 0.f;
+    const float g = GUIDED ? c.guidance[row] : 0.f;
     const float rho = c.repetition ? c.repetition[row] : 1.f, pres = c.presence ? c.presence[row] : 0.f, freq = c.frequency ? c.frequency[row] : 0.f;
 #pragma unroll
     for (int j = 0; j < LC_GROUPS; ++j) {
         const int k = (j * LC_THREADS + tid) * 4, v = v0 + k, left = a.vocab - v;
         if (left <= 0) break;
-        if (a.uncond) {
+        if constexpr (GUIDED) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[j][i] = lc_mix(g, x[j][i], u[j][i]);
         }
@@ -258,10 +259,14 @@ extern "C" int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, i
     OpDevice dev((hipStream_t)stream, out);
     LC_TRY(dev.status());
     const dim3 grid = op_grid((uint64_t)a.groups * rows), block(LC_THREADS);
-    if (dtype == MV_F32 && out_dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<true, true>), grid, block, 0, (hipStream_t)stream, a);
-    else if (dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<true, false>), grid, block, 0, (hipStream_t)stream, a);
-    else if (out_dtype == MV_F32) hipLaunchKernelGGL((logit_controls_kernel<false, true>), grid, block, 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((logit_controls_kernel<false, false>), grid, block, 0, (hipStream_t)stream, a);
+    const auto launch = [&](auto in32, auto out32) {
+        if (uncond) hipLaunchKernelGGL((logit_controls_kernel<decltype(in32)::value, decltype(out32)::value, true>), grid, block, 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL((logit_controls_kernel<decltype(in32)::value, decltype(out32)::value, false>), grid, block, 0, (hipStream_t)stream, a);
+    };
+    if (dtype == MV_F32 && out_dtype == MV_F32) launch(std::true_type{}, std::true_type{});
+    else if (dtype == MV_F32) launch(std::true_type{}, std::false_type{});
+    else if (out_dtype == MV_F32) launch(std::false_type{}, std::true_type{});
+    else launch(std::false_type{}, std::false_type{});
     LC_TRY(hipGetLastError());
     return MV_OK;
 }
