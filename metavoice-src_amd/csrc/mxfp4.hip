@@ -34,7 +34,8 @@ namespace {
 
 // ---- quantiser --------------------------------------------------------------------------------------------------------------------------
 // One thread: 8 columns; the 4 threads of a quad share a block and its largest magnitude by two lane moves: no LDS, no second pass.  Memory bound: 28672 x
-// 8192 fp32 in 266 us, 5.8 TB/s (a large copy: 5.1); 2562 x 2048 bf16 with the dequantised copy in 6.2 us, where a launch's latency shows.
+// 8192 fp32 in 269 us, 5.7 TB/s (a large copy: 5.1); 2562 x 2048 bf16 with the dequantised copy in 6.3 us, where a launch's latency shows; 2 .. 256 rows of
+// activations 2 - 3 us, 2048 x 5632 5.3 us.
 struct QuantArgs {
     const void* w;
     unsigned char* codes;
@@ -132,28 +133,29 @@ __device__ __forceinline__ float mx_silu_bf16(float v) { return v / (1.0f + __ex
 __device__ __forceinline__ float mx_silu_f32(float v) { return v / (1.0f + expf(-v)); }
 
 // y = x . w + bias (gated: silu(y) * (x . w2 + bias2)) + residual, in fp32, rounded once
+template <bool GATED>
 __device__ __forceinline__ void mx_store(const MxArgs& a, int m, int n, float v, float v2) {
     if (a.bias) v += bf2f(a.bias[n]);
-    if (a.w2) {
-        if (a.bias2) v2 += bf2f(a.bias2[n]);
-        v = (a.out_f32 ? mx_silu_f32(v) : mx_silu_bf16(v)) * v2;
-    }
+    if (GATED && a.bias2) v2 += bf2f(a.bias2[n]);
     const int64_t at = (int64_t)m * a.N + n;
     if (a.out_f32) {
+        if (GATED) v = mx_silu_f32(v) * v2;
         if (a.res) v += ((const float*)a.res)[at];
         ((float*)a.out)[at] = v;
     } else {
+        if (GATED) v = mx_silu_bf16(v) * v2;
         if (a.res) v += bf2f(((const bf16_t*)a.res)[at]);
         ((bf16_t*)a.out)[at] = f2bf(v);
     }
 }
 
 // mx_store for 8 consecutive columns
+template <bool GATED>
 __device__ __forceinline__ void mx_store8(const MxArgs& a, int m, int n, float (&v)[8], float (&v2)[8]) {
     if (n + 8 > a.N) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (n + e < a.N) mx_store(a, m, n + e, v[e], v2[e]);
+            if (n + e < a.N) mx_store<GATED>(a, m, n + e, v[e], v2[e]);
         return;
     }
     if (a.bias) {
@@ -161,23 +163,20 @@ __device__ __forceinline__ void mx_store8(const MxArgs& a, int m, int n, float (
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += e & 1 ? bf_hi(b[e >> 1]) : bf_lo(b[e >> 1]);
     }
-    if (a.w2) {
-        if (a.bias2) {
-            const u32x4 b = *(const u32x4_any*)(a.bias2 + n);
+    if (GATED && a.bias2) {
+        const u32x4 b = *(const u32x4_any*)(a.bias2 + n);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v2[e] += e & 1 ? bf_hi(b[e >> 1]) : bf_lo(b[e >> 1]);
-        }
-        if (!a.out_f32) {  // fp32: below
+        for (int e = 0; e < 8; ++e) v2[e] += e & 1 ? bf_hi(b[e >> 1]) : bf_lo(b[e >> 1]);
+    }
+    if (GATED && !a.out_f32) {  // here and not beside the stores of bf16, where it costs 512 x 11008 x 4096 4 %
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = mx_silu_bf16(v[e]) * v2[e];
-        }
+        for (int e = 0; e < 8; ++e) v[e] = mx_silu_bf16(v[e]) * v2[e];
     }
     const int64_t at = (int64_t)m * a.N + n;
     if (a.out_f32) {
-        if (a.w2) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = mx_silu_f32(v[e]) * v2[e];
-        }
+        for (int e = 0; e < 8; ++e)
+            if (GATED) v[e] = mx_silu_f32(v[e]) * v2[e];
         if (a.res) {
             const f32x4_any lo = *(const f32x4_any*)((const float*)a.res + at), hi = *(const f32x4_any*)((const float*)a.res + at + 4);
 #pragma unroll
@@ -221,13 +220,13 @@ __device__ __forceinline__ bf16x8_t mx_widen(uint32_t q, float scale) {
 // Few rows: one workgroup computes 16 MT rows of x against 16 NT weight rows; its waves take steps of K in turn, each straight from memory to registers,
 // and their sums meet in LDS, in wave order.  The weights are the first operand of the matrix instruction, so a lane ends with 4 consecutive output
 // columns of one row.  Bound by the cache lines that a CU reads, or by latency when the matrix is small: bf16 rows 2 x 2562 x 2048 4.1 us, 16 x 5632 x 2048
-// gated 9.0 us (1.4 TB/s), codes 16 x 2048 x 5632 5.6 us.
+// gated 9.3 us (1.35 TB/s), codes 16 x 2048 x 5632 5.7 us.
 // LINES, where all rows begin on a 128-byte line: a step is 256 columns and a load of a wave covers 8 rows x 128 bytes.  Lane (r = lane & 15, g =
 // lane >> 4) reads row r & 7 (a second load: 8 + (r & 7)), piece g + 4 (r >> 3) of 16 bytes; mx_pair turns two such loads into the two halves of the
 // 128 bytes in operand order: row r, pieces g and 4 + g.
 // Without it a step is 128 columns and the lane reads block g of row r, which is its operand already.  On whole lines the first is 5 - 8 % faster with
-// bf16 rows and 10 - 25 % with codes (16 x 16384 x 8192: 25.3 -> 23.2 us, 21.6 -> 18.3 us); on rows that straddle lines it loses 10 - 25 % (16 x 4096 x
-// 4064: 5.8 -> 6.3 us, 4.4 -> 5.0 us).
+// bf16 rows (16 x 16384 x 8192: 25.3 -> 23.2 us) and 10 - 25 % with codes; on rows that straddle lines it loses 10 - 25 % (16 x 4096 x 4064: 5.8 -> 6.3 us,
+// codes 4.4 -> 5.0 us).
 __device__ __forceinline__ void mx_pair(u32x4& a, u32x4& b) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // rotated by 8 within 16 lanes; lanes 8 .. 15 of the first, 0 .. 7 of the second half
@@ -370,13 +369,13 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
             v += sums[w * TILES * 256 + at];
             if (GATED) v2 += sums[w * TILES * 256 + NT * MT * 256 + at];
         }
-        if (m0 + row < a.M && n0 + c < a.N) mx_store(a, m0 + row, n0 + c, v, v2);
+        if (m0 + row < a.M && n0 + c < a.N) mx_store<GATED>(a, m0 + row, n0 + c, v, v2);
     }
 }
 
 // ---- large products -----------------------------------------------------------------------------------------------------------------------
 // One workgroup computes BM rows of x against BN weight rows, a wave 32 TX x 32 TW of them on 32x32 matrix instructions with the weights as the first
-// operand (a lane ends with 4 consecutive output columns of one row).  K advances in stages: 64 bf16 (128 bytes) or 128 codes (64 bytes) of a row.
+// operand (a lane ends with 4 consecutive output columns of one row).  K advances in stages: 64 bf16 or 256 codes (128 bytes) of a row per team.
 // Lane (r = lane & 31, h = lane >> 5) takes 16-byte chunk STEPS h + t of its row at step t.  With codes its steps are consecutive blocks: their scales
 // lie side by side and byte t of one register serves step t.  With bf16 its 4 steps are one block of its weight row: one 16-byte read of codes that it
 // widens 8 at a time.
@@ -386,13 +385,16 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
 // Scales come 16 blocks of a row at a time, a group ahead, two groups in LDS (a few bytes per row and stage would touch as many cache lines as the
 // codes do).
 // LDS has 64 banks and serves 16 lanes of a 16-byte read at a time: chunk c of a row lies at c ^ (row / (rows per 256 bytes)), so 16 rows
-// spread over all banks.  A transfer writes LDS in lane order: the permutation is applied to the lane's address in memory.
+// spread over all banks.  A transfer writes LDS in lane order: the permutation is applied to the lane's address in memory.  The scales are not spread: their
+// reads (1 or 4 bytes of rows 16 bytes apart) are the bank conflicts that the counters show, 6 cycles each: 29 % of the LDS cycles with bf16 rows, 23 % with
+// codes.
 // Five tiles, the smaller ones for grids that would leave CUs idle: 256 x 256 (8 waves of 64 rows x 128 columns) and 128 x 256 (8 of 64 x 64); with the waves
 // in teams that split a stage's columns 128 x 128 and 64 x 128 (two teams of 4 waves) and 64 x 64 (bf16 rows: four teams of 2, codes: two of 4).
 // Measured: 64 x 16384 x 8192 by the last one bf16 rows 27 us (128 x 128: 57), codes 15 us (24), the weights at 4.7 TB/s; 384 x 16384 x 8192 by 128 x 256
-// codes 38 us (47), bf16 rows 108 us (121); by 256 x 256 bf16 rows 4096 x 16384 x 8192 in 840 us, 1.31 PFLOP/s (a library product of two bf16 matrices:
-// 704 us), codes 8192 x 16384 x 8192 in 560 us, 3.9 PFLOP/s.  The last two are bound by power: the matrix units are busy 68 % (bf16) and 57 % (codes) of
-// the time at 1.8 GHz, and a loop of the same matrix instructions alone, on the same data in registers, takes 685 us and 2 x 216 us.
+// codes 41 us (128 x 128: 48), bf16 rows 118 us (121); by 256 x 256, medians, bf16 rows 4096 x 16384 x 8192 in 928 us, 1.18 PFLOP/s (fastest 867; a library
+// product of two bf16 matrices: 721 us), codes 8192 x 16384 x 8192 in 600 us, 3.7 PFLOP/s (fastest 573).  The last two are bound by power: the matrix units are
+// busy 67 % (bf16) and 56 % (codes) of the time at 1.8 GHz, and a loop of the same matrix instructions alone, on operands of the same distribution in
+// registers, takes 660 us and 2 x 194 us.
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* glb_ptr_t;
@@ -814,7 +816,7 @@ __global__ void __launch_bounds__(64 * KS * WN * WM, 2) mx_tile_kernel(const MxA
                 v[e] = et[row * PITCH + c8 + e];
                 v2[e] = GATED ? et[row * PITCH + OUT + c8 + e] : 0.f;
             }
-            mx_store8(a, m, n, v, v2);
+            mx_store8<GATED>(a, m, n, v, v2);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
@@ -857,10 +859,11 @@ hipError_t launch_rows(hipStream_t s, MxArgs a) {
     return hipGetLastError();
 }
 
-// Estimated microseconds of the two kernels, in the coefficients that a fit to 602 sets of measured products gives (1 .. 2048 rows, 100 .. 16384 columns,
-// K from 300 to 11008; the choice by them costs 1 % over the best one on average, and without one of the five tiles 2 - 7 %).  A workgroup of the first
-// kernel reads its rows of x and of the weights; what counts is how much the busiest CU reads (workgroups with 4 and more products share one unevenly:
-// rounds of them count).  One of the second advances by stages, a little slower when all CUs work, 1.4 times as long where scales come through registers.
+// Estimated microseconds of the two kernels, in coefficients fitted to 602 measured calls (1 .. 4096 rows, 100 .. 16384 columns, K from 300 to 11008; beyond
+// that they are carried on).  Over these the choice costs 1 % over the best kernel on average (at most 43 %: 192 x 400 x 8192), and 2.5 - 10 % without any one
+// of the five tiles; the estimate itself is off by 5 % in the middle and 39 % at most.  A workgroup of the first kernel reads its rows of x and of the weights;
+// what counts is how much the busiest CU reads (workgroups with 4 and more products share one unevenly: rounds of them count).  One of the second advances by
+// stages, a little slower when all CUs work, 1.4 times as long where scales come through registers.
 template <bool X4>
 double rows_us(const MxArgs& a, int mt, int nt) {
     const double mats = a.w2 ? 2 : 1, products = mt * nt * mats, per_cu = (double)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt)) / 256;

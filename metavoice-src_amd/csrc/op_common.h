@@ -1,4 +1,4 @@
-// Host-side helpers of the stand-alone operators (mxfp4.hip, logits.hip): error reporting and the device a call works on.
+// Helpers of the stand-alone operators (mxfp4.hip, logits.hip): error reporting, the device a call works on, grids, buffers that overlap, a fast division.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -88,7 +88,7 @@ inline bool op_overlap(const OpRows& a, const OpRows& b) {
     return false;
 }
 
-// n / d for 0 <= n < 2^31 by a multiply and a shift
+// n / d for 0 <= n < 2^31 by a multiply and a shift: the division by an invariant of Granlund and Montgomery (1994), mul = 2^32 (2^shift - d) / d + 1
 struct FastDiv {
     uint32_t mul = 0, shift = 0, d = 1;
     FastDiv() = default;
