@@ -98,3 +98,16 @@ def test_rows_far_apart(stride, tiled):
     within(out, want, size, k, torch.float32)
     del room, x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("kind,kernel,gated,form,x_direct,m,n,k,pad", [c for c in CASES if c[0] == "linear" and c[4] == 1])
+def test_nan_between_rows_of_x(kind, kernel, gated, form, x_direct, m, n, k, pad):
+    """What lies between the rows of x and behind the last one is not read, or not used: NaN there, beside a K that ends inside a block."""
+    k -= 5 if k % 32 == 0 else 0
+    ld = (k + 127) // 64 * 64 + (0 if kernel > 2 or form else 2)
+    args, want, size = case("linear", m, n, k, bool(gated), False, False, torch.float32, make=make_fast)
+    room = torch.full((m + 1, ld), float("nan"), dtype=torch.bfloat16, device="cuda")
+    room[:m, :k] = args["x"]
+    args["x"] = room[:m, :k]
+    assert reaches(chosen("linear", m, n, k, gated, ld, room.data_ptr()), kernel, form, x_direct)
+    within(product("linear", **args), want, size, k, torch.float32)
