@@ -149,8 +149,9 @@ int mv_op_quantize_mxfp4(void* stream, int32_t N, int32_t K, int32_t dtype, cons
                          void* dequantised);
 /* out[M][N] = x . W^T + bias, with codes2 / scales2 the gated pair silu(x . W^T + bias) * (x . W2^T + bias2); then + residual.  x bf16 [M][ldx];
  * W, W2 MXFP4 [N][K]; bias, bias2 bf16 [N] or NULL; residual [M][N] of the output's type or NULL (may be `out` itself); out_dtype MV_BF16 or
- * MV_F32.  The weights enter the matrix cores as bf16 (exact), sums are fp32, the result is rounded once.  The kernel is chosen by the sizes, so a
- * row's last bits may differ between calls of different M; equal calls give equal bits. */
+ * MV_F32.  The weights enter the matrix cores as bf16 (exact), sums are fp32, the result is rounded once.  The kernel is chosen by the sizes, the
+ * stride of x and how the buffers are aligned, so a row's last bits may differ between calls of different M or alignment; equal calls give equal
+ * bits. */
 int mv_op_linear_mxfp4(void* stream, int32_t M, int32_t N, int32_t K, const void* x, int64_t ldx, const void* codes, const void* scales,
                        const void* codes2, const void* scales2, const void* bias, const void* bias2, const void* residual, int32_t out_dtype,
                        void* out);
@@ -196,8 +197,8 @@ typedef struct mv_logit_controls {
  * (same dtype and stride); else outputs lie apart from inputs and from each other (calls where they share a byte are refused, but for interleaved
  * rows of two different strides).  allowed (optional) [rows]: tokens the mask leaves, 0 when a grammar has run into a dead end (the row is -inf
  * throughout).
- * Enqueued on `stream`: no allocation, no scratch memory, no synchronisation.  out feeds mv_op_sample with a row of zeros as the unconditioned
- * logits, guidance_scale 1, one_minus_guidance 0. */
+ * Enqueued on `stream`: no allocation, no scratch memory, no synchronisation.  out feeds mv_op_sample (bf16, at most 4096 tokens; it
+ * synchronises, so a captured step ends before the draw) with a row of zeros as the unconditioned logits, guidance_scale 1, one_minus_guidance 0. */
 int mv_op_logit_controls(void* stream, int32_t rows, int32_t vocab, int32_t dtype, const void* logits, const void* uncond, int64_t ld,
                          const mv_logit_controls* controls, int32_t out_dtype, void* out, int64_t ld_out, int32_t* allowed);
 

@@ -11,8 +11,8 @@
 // the bias entry that holds.  It scans the whole history and bias list of its row and keeps what falls into its chunk: a history is short beside the
 // row (and comes from the L2 for all chunks but the first), so this replaces a count array in memory, a launch that clears it and one that fills it.
 // Integer adds, ors and maxima in LDS give the same words in any order: results do not depend on timing.  Bound by memory when rows x vocab is large,
-// by the latency of one launch with two dependent loads (length, then history) when it is not: 256 x 131072 fp32 in 55 us, 4.9 TB/s (a large copy: 5.1); 64 x
-// 32003 bf16 to fp32 with histories of 4096 10 us; 1 x 2562 4.4 us.
+// by the latency of one launch with two dependent loads (length, then history) when it is not: 256 x 131072 fp32 in 54 us, 5.0 TB/s (a large copy: 5.1); 64 x
+// 32003 bf16 to fp32 with histories of 4096 9.0 us; 1 x 2562 4.8 us.
 #include "common.h"
 #include "op_common.h"
 

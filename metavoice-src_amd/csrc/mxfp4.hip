@@ -34,7 +34,7 @@ namespace {
 
 // ---- quantiser --------------------------------------------------------------------------------------------------------------------------
 // One thread: 8 columns; the 4 threads of a quad share a block and its largest magnitude by two lane moves: no LDS, no second pass.  Memory bound: 28672 x
-// 8192 fp32 in 269 us, 5.7 TB/s (a large copy: 5.1); 2562 x 2048 bf16 with the dequantised copy in 6.3 us, where a launch's latency shows; 2 .. 256 rows of
+// 8192 fp32 in 268 us, 5.7 TB/s (a large copy: 5.1); 2562 x 2048 bf16 with the dequantised copy in 6.3 us, where a launch's latency shows; 2 .. 256 rows of
 // activations 2 - 3 us, 2048 x 5632 5.3 us.
 struct QuantArgs {
     const void* w;
@@ -220,7 +220,7 @@ __device__ __forceinline__ bf16x8_t mx_widen(uint32_t q, float scale) {
 // Few rows: one workgroup computes 16 MT rows of x against 16 NT weight rows; its waves take steps of K in turn, each straight from memory to registers,
 // and their sums meet in LDS, in wave order.  The weights are the first operand of the matrix instruction, so a lane ends with 4 consecutive output
 // columns of one row.  Bound by the cache lines that a CU reads, or by latency when the matrix is small: bf16 rows 2 x 2562 x 2048 4.1 us, 16 x 5632 x 2048
-// gated 9.3 us (1.35 TB/s), codes 16 x 2048 x 5632 5.7 us.
+// gated 9.2 us (1.36 TB/s), codes 16 x 2048 x 5632 5.8 us.
 // LINES, where all rows begin on a 128-byte line: a step is 256 columns and a load of a wave covers 8 rows x 128 bytes.  Lane (r = lane & 15, g =
 // lane >> 4) reads row r & 7 (a second load: 8 + (r & 7)), piece g + 4 (r >> 3) of 16 bytes; mx_pair turns two such loads into the two halves of the
 // 128 bytes in operand order: row r, pieces g and 4 + g.
@@ -391,10 +391,10 @@ __global__ void __launch_bounds__(64 * MX_WAVES, 2) mx_rows_kernel(const MxArgs 
 // Five tiles, the smaller ones for grids that would leave CUs idle: 256 x 256 (8 waves of 64 rows x 128 columns) and 128 x 256 (8 of 64 x 64); with the waves
 // in teams that split a stage's columns 128 x 128 and 64 x 128 (two teams of 4 waves) and 64 x 64 (bf16 rows: four teams of 2, codes: two of 4).
 // Measured: 64 x 16384 x 8192 by the last one bf16 rows 27 us (128 x 128: 57), codes 15 us (24), the weights at 4.7 TB/s; 384 x 16384 x 8192 by 128 x 256
-// codes 41 us (128 x 128: 48), bf16 rows 118 us (121); by 256 x 256, medians, bf16 rows 4096 x 16384 x 8192 in 928 us, 1.18 PFLOP/s (fastest 867; a library
-// product of two bf16 matrices: 721 us), codes 8192 x 16384 x 8192 in 600 us, 3.7 PFLOP/s (fastest 573).  The last two are bound by power: the matrix units are
-// busy 67 % (bf16) and 56 % (codes) of the time at 1.8 GHz, and a loop of the same matrix instructions alone, on operands of the same distribution in
-// registers, takes 660 us and 2 x 194 us.
+// codes 41 us (128 x 128: 48), bf16 rows 115 us (121); by 256 x 256, medians, bf16 rows 4096 x 16384 x 8192 in 925 us, 1.19 PFLOP/s (fastest 850; a library
+// product of two bf16 matrices: 713 us), codes 8192 x 16384 x 8192 in 608 us, 3.6 PFLOP/s (fastest 557).  The last two are bound by power: the matrix units are
+// busy 68 % (bf16) and 57 % (codes) of the time at about 1.8 GHz, and a loop of the same matrix instructions alone, on operands of the same distribution in
+// registers, takes 658 us and 2 x 198 us.
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* glb_ptr_t;
